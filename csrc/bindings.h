@@ -7,6 +7,8 @@ namespace engram {
 
 // ops.cpp: the standalone per-owner pack and the NVTX switch.
 void bind_ops(pybind11::module_ &m);
+// readout.cpp: layer norm, 8-bit activation checkpoints and a projection's gradients.
+void bind_readout(pybind11::module_ &m);
 // harness.cpp: CPU harnesses for the owner service and descriptor passing.
 void bind_harness(pybind11::module_ &m);
 

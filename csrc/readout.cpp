@@ -1,0 +1,351 @@
+// Read-out operators of the extension: layer norm over looked-up rows, 8-bit
+// activation checkpoints, and a projection's gradients from such a checkpoint.
+// Arguments are checked here (ValueError, before any device is touched);
+// everything runs on the current stream of the inputs' device, and outputs and
+// workspaces come from torch's allocator, so calls can be captured into graphs.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <pybind11/stl.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <string>
+
+#include "bindings.h"
+#include "driver.h"
+#include "kernels/readout.h"
+
+namespace py = pybind11;
+
+namespace engram {
+
+namespace {
+
+using at::ScalarType;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+void need(bool ok, const char *what) {
+    if (!ok)
+        throw py::value_error(what);
+}
+
+bool is_wide(ScalarType t) {
+    return t == ScalarType::BFloat16 || t == ScalarType::Half || t == ScalarType::Float;
+}
+
+uint32_t element_type(ScalarType t) {
+    return t == ScalarType::BFloat16 ? kBf16 : t == ScalarType::Half ? kFp16 : t == ScalarType::Float ? kFp32 : kE4m3;
+}
+
+// [rows, width] with adjacent columns; rows may be strided (0: repeated).
+void need_rows(const Tensor &t, const char *what) {
+    need(t.dim() == 2 && t.size(1) >= 1 && t.size(1) <= (1 << 30) && t.size(0) <= 0x7FFFFFFF &&
+             (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= 0,
+         what);
+}
+
+// Per-column parameters of a norm: [width], 16-bit like the rows or fp32.
+void need_params(const OptTensor &weight, const OptTensor &bias, int64_t width, ScalarType rows_type) {
+    need(!bias || weight, "a bias needs a weight");
+    if (!weight)
+        return;
+    need(weight->dim() == 1 && weight->size(0) == width && weight->is_contiguous(), "weight must be contiguous [width]");
+    need(weight->scalar_type() == rows_type || weight->scalar_type() == ScalarType::Float,
+         "weight must have the rows' type or float32");
+    if (bias)
+        need(bias->dim() == 1 && bias->size(0) == width && bias->is_contiguous() &&
+                 bias->scalar_type() == weight->scalar_type(),
+             "bias must be contiguous [width] of the weight's type");
+}
+
+// A checkpoint's codes [rows, width] and scales [rows, ceil(width / 128)].
+void need_checkpoint(const Tensor &codes, const Tensor &scales) {
+    need_rows(codes, "codes must be [rows, width] with adjacent columns");
+    need(codes.scalar_type() == ScalarType::Float8_e4m3fn, "codes must be float8_e4m3fn");
+    need(scales.dim() == 2 && scales.scalar_type() == ScalarType::Float && scales.size(0) == codes.size(0) &&
+             scales.size(1) == (codes.size(1) + kCheckpointBlock - 1) / kCheckpointBlock,
+         "scales must be float32 [rows, ceil(width / 128)]");
+}
+
+// The device all of these are on, which has to be a GPU.
+int need_device(const Tensor &first, std::initializer_list<const OptTensor *> others) {
+    need(first.is_cuda(), "tensors must be on a GPU");
+    for (const OptTensor *t : others)
+        need(!*t || (*t)->device() == first.device(), "tensors must be on one GPU");
+    return first.get_device();
+}
+
+int sm_count(int device) { return at::cuda::getDeviceProperties(device)->multiProcessorCount; }
+
+void *data(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
+
+// Code rows start on 16-byte boundaries, so every kernel can read them in vectors.
+Tensor empty_codes(const Tensor &like, int64_t rows, int64_t width) {
+    return at::empty({rows, (width + 15) / 16 * 16}, like.options().dtype(ScalarType::Float8_e4m3fn)).narrow(1, 0, width);
+}
+
+Tensor empty_scales(const Tensor &like, int64_t rows, int64_t width) {
+    return at::empty({rows, (width + kCheckpointBlock - 1) / kCheckpointBlock}, like.options().dtype(ScalarType::Float));
+}
+
+// (y, codes | None, scales | None, mean | None, rstd | None)
+py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps,
+                       const OptTensor &scales, std::optional<int64_t> hidden, int64_t block,
+                       std::optional<ScalarType> dtype, uint32_t keep) {
+    need_rows(x, "rows must be [tokens, width] with adjacent columns");
+    const int64_t rows = x.size(0), width = x.size(1);
+    const bool fp8 = x.scalar_type() == ScalarType::Float8_e4m3fn;
+    need(fp8 || is_wide(x.scalar_type()), "rows must be bfloat16, float16, float32 or float8_e4m3fn");
+    const ScalarType out = fp8 ? dtype.value_or(ScalarType::BFloat16) : x.scalar_type();
+    need(is_wide(out), "dtype must be bfloat16, float16 or float32");
+    need(fp8 || !dtype || *dtype == out, "dtype can be chosen for float8_e4m3fn rows only");
+    need(fp8 == scales.has_value(), "float8_e4m3fn rows need scales, other rows take none");
+    need(eps >= 0, "eps must not be negative");
+    need(keep <= kKeepFp8 && !(fp8 && keep == kKeepStats), "float8_e4m3fn rows are kept as \"fp8\" only");
+    NormForwardParams p{};
+    p.hidden = uint32_t(hidden.value_or(width));
+    if (fp8) {
+        const int64_t h = hidden.value_or(width);
+        need(h >= 1 && h <= width && width % h == 0, "hidden must divide the width");
+        need(block >= 1 && block <= (1 << 30), "block must be positive");
+        const int64_t packs = (h + block - 1) / block;
+        need(scales->dim() == 2 && scales->scalar_type() == ScalarType::Float && scales->size(0) == rows &&
+                 scales->size(1) == width / h * packs,
+             "scales must be float32 [tokens, width / hidden * ceil(hidden / block)]");
+        p.scales = static_cast<const float *>(scales->data_ptr());
+        p.scale_row_stride = scales->stride(0);
+        p.scale_col_stride = scales->stride(1);
+        p.packs = uint32_t(packs);
+        p.block = uint32_t(block);
+    } else {
+        need(!hidden, "hidden describes the scales of float8_e4m3fn rows");
+    }
+    need_params(weight, bias, width, out);
+    const int device = need_device(x, {&weight, &bias, &scales});
+    c10::cuda::CUDAGuard guard(device);
+    const Tensor y = at::empty({rows, width}, x.options().dtype(out));
+    OptTensor codes, code_scales, mean, rstd;
+    if (keep != kKeepNothing)
+        rstd = at::empty({rows}, x.options().dtype(ScalarType::Float));
+    if (keep == kKeepStats)
+        mean = at::empty({rows}, x.options().dtype(ScalarType::Float));
+    if (keep == kKeepFp8) {
+        codes = empty_codes(x, rows, width);
+        code_scales = empty_scales(x, rows, width);
+    }
+    if (rows > 0) {
+        p.x = x.data_ptr();
+        p.weight = data(weight);
+        p.bias = data(bias);
+        p.y = y.data_ptr();
+        p.mean = static_cast<float *>(data(mean));
+        p.rstd = static_cast<float *>(data(rstd));
+        p.codes = static_cast<uint8_t *>(data(codes));
+        p.code_scales = static_cast<float *>(data(code_scales));
+        p.rows = rows;
+        p.x_stride = x.stride(0);
+        p.codes_stride = codes ? codes->stride(0) : 0;
+        p.width = uint32_t(width);
+        p.in_type = element_type(x.scalar_type());
+        p.out_type = element_type(out);
+        p.param_type = weight ? element_type(weight->scalar_type()) : 0;
+        p.keep = keep;
+        p.eps = float(eps);
+        check_cuda(launch_norm_forward(p, sm_count(device), at::cuda::getCurrentCUDAStream(device).stream()),
+                   "launch layer norm");
+    }
+    return py::make_tuple(y, codes, code_scales, mean, rstd);
+}
+
+// (dx | None, dweight | None, dbias | None).  Kept rows: (x, mean, rstd) or (codes, scales, rstd).
+py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &scales, const OptTensor &mean,
+                        const Tensor &rstd, const OptTensor &weight, bool want_dx, bool want_params) {
+    need_rows(dy, "dy must be [tokens, width] with adjacent columns");
+    need(is_wide(dy.scalar_type()), "dy must be bfloat16, float16 or float32");
+    const int64_t rows = dy.size(0), width = dy.size(1);
+    const bool fp8 = scales.has_value();
+    need(kept.dim() == 2 && kept.size(0) == rows && kept.size(1) == width, "dy must have the shape of the kept rows");
+    if (fp8) {
+        need_checkpoint(kept, *scales);
+    } else {
+        need_rows(kept, "rows must be [tokens, width] with adjacent columns");
+        need(kept.scalar_type() == dy.scalar_type(), "dy must have the rows' type");
+        need(mean && mean->dim() == 1 && mean->size(0) == rows && mean->scalar_type() == ScalarType::Float &&
+                 mean->is_contiguous(),
+             "mean must be contiguous float32 [tokens]");
+    }
+    need(rstd.dim() == 1 && rstd.size(0) == rows && rstd.scalar_type() == ScalarType::Float && rstd.is_contiguous(),
+         "rstd must be contiguous float32 [tokens]");
+    need_params(weight, std::nullopt, width, dy.scalar_type());
+    const OptTensor kept_opt = kept, rstd_opt = rstd;
+    const int device = need_device(dy, {&kept_opt, &scales, &mean, &rstd_opt, &weight});
+    c10::cuda::CUDAGuard guard(device);
+    OptTensor dx, dweight, dbias, partial;
+    if (want_dx)
+        dx = at::empty({rows, width}, dy.options());
+    const bool params = want_params && weight.has_value();
+    if (params) {
+        dweight = at::empty({width}, weight->options());
+        dbias = at::empty({width}, weight->options());
+    }
+    if (rows == 0) {
+        if (params) {
+            dweight->zero_();
+            dbias->zero_();
+        }
+        return py::make_tuple(dx, dweight, dbias);
+    }
+    NormBackwardParams p{};
+    p.dy = dy.data_ptr();
+    p.rstd = static_cast<const float *>(rstd.data_ptr());
+    if (fp8) {
+        p.codes = static_cast<const uint8_t *>(kept.data_ptr());
+        p.code_scales = static_cast<const float *>(scales->data_ptr());
+        p.codes_stride = kept.stride(0);
+        p.code_scales_stride = scales->stride(0);
+        p.scale_col_stride = scales->stride(1);
+    } else {
+        p.x = kept.data_ptr();
+        p.x_stride = kept.stride(0);
+        p.mean = static_cast<const float *>(mean->data_ptr());
+    }
+    p.weight = data(weight);
+    p.dx = data(dx);
+    p.dweight = data(dweight);
+    p.dbias = data(dbias);
+    p.rows = rows;
+    p.dy_stride = dy.stride(0);
+    p.width = uint32_t(width);
+    p.dy_type = element_type(dy.scalar_type());
+    p.x_type = element_type(kept.scalar_type());
+    p.param_type = weight ? element_type(weight->scalar_type()) : 0;
+    p.keep = fp8 ? kKeepFp8 : kKeepStats;
+    const int sms = sm_count(device);
+    if (params) {
+        p.parts = norm_backward_parts(p, sms);
+        partial = at::empty({2, int64_t(p.parts), width}, dy.options().dtype(ScalarType::Float));
+        p.partial = static_cast<float *>(partial->data_ptr());
+    }
+    check_cuda(launch_norm_backward(p, sms, at::cuda::getCurrentCUDAStream(device).stream()),
+               "launch layer norm backward");
+    return py::make_tuple(dx, dweight, dbias);
+}
+
+py::tuple save_fp8(const Tensor &x) {
+    need_rows(x, "activations must be [rows, width] with adjacent columns");
+    need(is_wide(x.scalar_type()), "activations must be bfloat16, float16 or float32");
+    const int device = need_device(x, {});
+    c10::cuda::CUDAGuard guard(device);
+    const int64_t rows = x.size(0), width = x.size(1);
+    const Tensor codes = empty_codes(x, rows, width), scales = empty_scales(x, rows, width);
+    if (rows > 0) {
+        SaveFp8Params p{};
+        p.x = x.data_ptr();
+        p.codes = static_cast<uint8_t *>(codes.data_ptr());
+        p.scales = static_cast<float *>(scales.data_ptr());
+        p.rows = rows;
+        p.x_stride = x.stride(0);
+        p.codes_stride = codes.stride(0);
+        p.width = uint32_t(width);
+        p.type = element_type(x.scalar_type());
+        check_cuda(launch_save_fp8(p, sm_count(device), at::cuda::getCurrentCUDAStream(device).stream()),
+                   "launch 8-bit save");
+    }
+    return py::make_tuple(codes, scales);
+}
+
+Tensor restore_fp8(const Tensor &codes, const Tensor &scales, ScalarType dtype) {
+    need_checkpoint(codes, scales);
+    need(is_wide(dtype), "dtype must be bfloat16, float16 or float32");
+    const OptTensor scales_opt = scales;
+    const int device = need_device(codes, {&scales_opt});
+    c10::cuda::CUDAGuard guard(device);
+    const int64_t rows = codes.size(0), width = codes.size(1);
+    const Tensor x = at::empty({rows, width}, codes.options().dtype(dtype));
+    if (rows > 0) {
+        RestoreFp8Params p{};
+        p.codes = static_cast<const uint8_t *>(codes.data_ptr());
+        p.scales = static_cast<const float *>(scales.data_ptr());
+        p.x = x.data_ptr();
+        p.rows = rows;
+        p.codes_stride = codes.stride(0);
+        p.scale_row_stride = scales.stride(0);
+        p.scale_col_stride = scales.stride(1);
+        p.width = uint32_t(width);
+        p.type = element_type(dtype);
+        check_cuda(launch_restore_fp8(p, sm_count(device), at::cuda::getCurrentCUDAStream(device).stream()),
+                   "launch 8-bit restore");
+    }
+    return x;
+}
+
+// (dweight [out, width], dbias [out] | None)
+py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &scales, const OptTensor &norm_weight,
+                          const OptTensor &norm_bias, std::optional<ScalarType> dtype, bool want_bias) {
+    need_rows(dy, "dy must be [rows, out] with adjacent columns");
+    need(is_wide(dy.scalar_type()), "dy must be bfloat16, float16 or float32");
+    need_checkpoint(codes, scales);
+    need(dy.size(0) == codes.size(0), "dy and codes must have the same rows");
+    const ScalarType result = dtype.value_or(dy.scalar_type());
+    need(result == dy.scalar_type() || result == ScalarType::Float, "dtype must be dy's type or float32");
+    const int64_t rows = dy.size(0), out = dy.size(1), width = codes.size(1);
+    need_params(norm_weight, norm_bias, width, dy.scalar_type());
+    const OptTensor codes_opt = codes, scales_opt = scales;
+    const int device = need_device(dy, {&codes_opt, &scales_opt, &norm_weight, &norm_bias});
+    c10::cuda::CUDAGuard guard(device);
+    const auto options = dy.options().dtype(result);
+    const Tensor dweight = at::empty({out, width}, options);
+    OptTensor dbias, sums, partial;
+    if (want_bias)
+        dbias = at::empty({out}, options);
+    if (rows == 0) {
+        dweight.zero_();
+        if (dbias)
+            dbias->zero_();
+        return py::make_tuple(dweight, dbias);
+    }
+    WeightGradParams p{};
+    p.dy = dy.data_ptr();
+    p.codes = static_cast<const uint8_t *>(codes.data_ptr());
+    p.scales = static_cast<const float *>(scales.data_ptr());
+    p.norm_weight = data(norm_weight);
+    p.norm_bias = data(norm_bias);
+    p.dweight = dweight.data_ptr();
+    p.dbias = data(dbias);
+    p.rows = rows;
+    p.dy_stride = dy.stride(0);
+    p.codes_stride = codes.stride(0);
+    p.scale_row_stride = scales.stride(0);
+    p.scale_col_stride = scales.stride(1);
+    p.width = uint32_t(width);
+    p.out = uint32_t(out);
+    p.type = element_type(dy.scalar_type());
+    p.param_type = norm_weight ? element_type(norm_weight->scalar_type()) : 0;
+    p.out_type = element_type(result);
+    const int sms = sm_count(device);
+    if (want_bias || norm_bias) {
+        p.parts = weight_grad_parts(p, sms);
+        sums = at::empty({out}, dy.options().dtype(ScalarType::Float));
+        partial = at::empty({int64_t(p.parts), out}, dy.options().dtype(ScalarType::Float));
+        p.dy_sums = static_cast<float *>(sums->data_ptr());
+        p.partial = static_cast<float *>(partial->data_ptr());
+    }
+    check_cuda(launch_weight_grad(p, sms, at::cuda::getCurrentCUDAStream(device).stream()), "launch weight gradient");
+    return py::make_tuple(dweight, dbias);
+}
+
+} // namespace
+
+void bind_readout(py::module_ &m) {
+    m.def("norm_forward", &norm_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),
+          py::arg("scales"), py::arg("hidden"), py::arg("block"), py::arg("dtype"), py::arg("keep"));
+    m.def("norm_backward", &norm_backward, py::arg("dy"), py::arg("kept"), py::arg("scales"), py::arg("mean"),
+          py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"));
+    m.def("save_fp8", &save_fp8, py::arg("x"));
+    m.def("restore_fp8", &restore_fp8, py::arg("codes"), py::arg("scales"), py::arg("dtype"));
+    m.def("fp8_weight_grad", &fp8_weight_grad, py::arg("dy"), py::arg("codes"), py::arg("scales"),
+          py::arg("norm_weight"), py::arg("norm_bias"), py::arg("dtype"), py::arg("want_bias"));
+}
+
+} // namespace engram

@@ -1500,5 +1500,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("close", &Runtime::close)
         .def_property_readonly("closed", &Runtime::closed);
     bind_ops(m);
+    bind_readout(m);
     bind_harness(m);
 }

@@ -10,9 +10,11 @@ from .engram_tables import (
     quantized_fp8_shard,
     row_pattern,
 )
+from .readout import EngramReadout
 
 __all__ = [
     "CONFIGS",
+    "EngramReadout",
     "TableSpec",
     "expected_outputs",
     "expected_random_init",

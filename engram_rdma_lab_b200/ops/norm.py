@@ -1,0 +1,103 @@
+"""Layer norm over looked-up rows, forward and backward (sm_100a kernels).
+
+The rows are what a lookup returns: ``[tokens, width]`` bf16 (fp16 and fp32 work too), or e4m3 codes with their
+scales, which the kernel multiplies in as it reads (no dequantised copy).  The backward pass reads what the forward
+pass kept: the rows themselves with two fp32 numbers per row (``keep="exact"``), or the normalised rows in 8 bits
+with one (``keep="fp8"``; the format of :mod:`.checkpoint`), half of bf16's bytes.  Normalised values are what suits
+8 bits: a row's common offset and size are gone before the rounding, so e4m3's relative precision is spent on what
+the gradient needs, and the same checkpoint serves the projection behind the norm
+(:func:`~.projection.fp8_weight_grad`).
+
+Sums over rows and columns are held in fp32 and joined in a fixed order: equal inputs give equal bits on equal GPUs.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+
+_KEEP = {None: 0, "exact": 1, "fp8": 2}
+
+
+class KeptRows(NamedTuple):
+    """What ``layer_norm_forward`` keeps: ``(x, None, mean, rstd)`` or ``(codes, scales, None, rstd)``."""
+
+    rows: torch.Tensor
+    scales: Optional[torch.Tensor]
+    mean: Optional[torch.Tensor]
+    rstd: torch.Tensor
+
+
+def _keep_mode(keep) -> int:
+    try:
+        return _KEEP[keep]
+    except (KeyError, TypeError):
+        raise ValueError('keep must be None, "exact" or "fp8"') from None
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hidden=None, block: int = 128,
+                       dtype=None, keep=None):
+    """``(y, kept)`` with ``y = (x - mean) / sqrt(var + eps) * weight + bias`` for each row of ``x [tokens, width]``.
+
+    ``x`` is bf16, fp16 or fp32 (``y`` has its type), or e4m3 codes with ``scales`` as ``fetch`` returns both:
+    ``scales [tokens, width // hidden * ceil(hidden / block)]`` fp32 of either layout, one per ``block`` columns of
+    each looked-up row of ``hidden`` columns (default: the width); ``y`` is then ``dtype`` (default bf16).
+    ``weight`` and ``bias [width]`` have y's type or are fp32.  ``keep`` says what the backward pass will read:
+    nothing (``kept`` is None), ``"exact"`` (``x`` itself, which must stay unchanged) or ``"fp8"``.  Codes of a lookup
+    are kept as ``"fp8"`` only: the next fetch reuses their memory.
+    """
+    mode = _keep_mode(keep)
+    y, codes, code_scales, mean, rstd = _native.load().norm_forward(
+        x, weight, bias, eps, scales, hidden, block, dtype, mode)
+    if mode == 0:
+        return y, None
+    return y, KeptRows(x, None, mean, rstd) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
+
+
+def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True, want_params: bool = True):
+    """``(dx, dweight, dbias)`` for the gradient ``dy [tokens, width]`` of ``layer_norm_forward``'s ``y``.
+
+    ``dx`` has dy's type (for looked-up codes it is the gradient of the dequantised rows), ``dweight`` and ``dbias``
+    the weight's type; both are None without a ``weight``.  What is not wanted is None and not computed.
+    """
+    return _native.load().norm_backward(dy, kept.rows, kept.scales, kept.mean, kept.rstd, weight, want_dx, want_params)
+
+
+def _adjacent(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, scales, hidden, block, dtype, keep):
+        y, kept = layer_norm_forward(x, weight, bias, eps, scales=scales, hidden=hidden, block=block, dtype=dtype,
+                                     keep=keep)
+        ctx.save_for_backward(*kept, weight)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, scales, mean, rstd, weight = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dweight, dbias = layer_norm_backward(_adjacent(dy), KeptRows(rows, scales, mean, rstd), weight,
+                                                 want_dx=need[0], want_params=need[1] or need[2])
+        return dx, dweight if need[1] else None, dbias if need[2] else None, None, None, None, None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hidden=None, block: int = 128, dtype=None,
+               keep: str = "fp8"):
+    """Differentiable layer norm of ``x [tokens, width]``; the arguments are :func:`layer_norm_forward`'s.
+
+    ``keep`` (``"fp8"`` or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
+    is wanted.  Looked-up e4m3 codes get no gradient themselves (:func:`layer_norm_backward` gives their rows').
+    """
+    if _keep_mode(keep) == 0:
+        raise ValueError('keep must be "exact" or "fp8"')
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, eps, scales, hidden, block, dtype, keep)
+    return layer_norm_forward(x, weight, bias, eps, scales=scales, hidden=hidden, block=block, dtype=dtype)[0]
