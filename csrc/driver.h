@@ -2,9 +2,10 @@
 //
 // The extension never links libcuda, so it imports on machines without a GPU
 // driver (the CPU unit tests) and always uses the driver that the CUDA runtime
-// already loaded.  Only the virtual-memory-management calls are needed: the
-// host shard and device arena are cuMemCreate allocations exported as POSIX
-// file descriptors and mapped by every peer on the node.
+// already loaded.  The virtual-memory-management calls are needed (the host
+// shard and device arena are cuMemCreate allocations exported as POSIX file
+// descriptors and mapped by every peer on the node), and the encoding of
+// tensor maps for tiled copies.
 #pragma once
 
 #include <cuda.h>
@@ -29,6 +30,7 @@ struct DriverApi {
     decltype(&::cuMemGetAllocationGranularity) MemGetAllocationGranularity = nullptr;
     decltype(&::cuDeviceGetAttribute) DeviceGetAttribute = nullptr;
     decltype(&::cuGetErrorString) GetErrorString = nullptr;
+    decltype(&::cuTensorMapEncodeTiled) TensorMapEncodeTiled = nullptr;
 };
 
 // Loads the table once; throws if the runtime cannot provide a symbol.

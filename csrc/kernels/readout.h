@@ -75,6 +75,7 @@ struct RestoreFp8Params {
 
 // dweight[o][k] = sum over rows of dy[row][o] * X[row][k], X the rows of an
 // 8-bit checkpoint; with a norm folded in, X * norm_weight + norm_bias.
+// Code rows, and bf16 dy rows, start on 16-byte boundaries.
 struct WeightGradParams {
     const void *dy;
     const uint8_t *codes;
@@ -82,9 +83,15 @@ struct WeightGradParams {
     const void *norm_weight, *norm_bias;  // nullptr: not folded
     void *dweight, *dbias;                // dbias nullptr: not wanted
     float *dy_sums;                       // [out] fp32 column sums of dy; nullptr: not needed
-    float *partial;                       // column-sum parts [parts][out]
-    int64_t rows, dy_stride, codes_stride, scale_row_stride, scale_col_stride;
-    uint32_t width, out, type, param_type, out_type, parts;
+    float *sum_parts;                     // [sum_rows][out]
+    void *dy_planes;                      // fp16, fp32: [planes][rows][plane_stride] bf16
+    float *dw_parts;                      // [parts][out][width], parts > 1
+    uint32_t *fault;                      // host-mapped: set when a wait ran out
+    int64_t rows, dy_stride, codes_stride, scale_row_stride, scale_col_stride, plane_stride;
+    uint32_t width, out, type, param_type, out_type, sum_rows;
+    // The plan (plan_weight_grad): dy as `planes` bf16 terms; blocks of `halves`
+    // x 128 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64.
+    uint32_t planes, halves, tile_k, tiles_k, tiles_o, parts, part_steps;
 };
 
 cudaError_t launch_norm_forward(const NormForwardParams &p, int num_sms, cudaStream_t stream);
@@ -93,7 +100,8 @@ uint32_t norm_backward_parts(const NormBackwardParams &p, int num_sms);
 cudaError_t launch_norm_backward(const NormBackwardParams &p, int num_sms, cudaStream_t stream);
 cudaError_t launch_save_fp8(const SaveFp8Params &p, int num_sms, cudaStream_t stream);
 cudaError_t launch_restore_fp8(const RestoreFp8Params &p, int num_sms, cudaStream_t stream);
-uint32_t weight_grad_parts(const WeightGradParams &p, int num_sms);
-cudaError_t launch_weight_grad(const WeightGradParams &p, int num_sms, cudaStream_t stream);
+// Fills in the plan and sum_rows from rows, width, out and type.
+void plan_weight_grad(WeightGradParams &p, int num_sms);
+cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream);
 
 } // namespace engram

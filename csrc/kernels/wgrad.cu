@@ -1,26 +1,36 @@
 // A projection's weight and bias gradients from the 8-bit checkpoint of its
-// input (sm_100a).
+// input (sm_100a, tcgen05).
 //
 // dW[o][k] = sum_m dy[m][o] X[m][k] with X the checkpoint's rows.  Where the
 // projection's input was X w + b (a norm's affine part), the same checkpoint
 // serves: dW[o][k] = w[k] G[o][k] + b[k] s[o], G = dy^T X and s[o] = sum_m
 // dy[m][o], which is also the bias gradient.
+//
+// X is decoded to bf16 on its way into shared memory, which is exact: a code
+// has four significant bits and its scale is a power of two.  dy is bf16, or a
+// sum of bf16 terms that hold every bit of it (two for fp16, three for fp32),
+// one more pass over the rows for each.  So all products are exact and only
+// the fp32 accumulation rounds.
+#include <algorithm>
+
+#include "../driver.h"
 #include "readout.h"
 #include "rowmath.cuh"
+#include "tensor.cuh"
 
 namespace engram {
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64, kDepth = 16;
 
-// Column sums of dy over one part of the rows.
+// ---------------------------------------------------------------- column sums of dy
+// Sums over one part of the rows: a block takes 32 columns.
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) dy_sums_part(const __grid_constant__ WeightGradParams p) {
     __shared__ float s_sum[kThreads / 32][32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, o = blockIdx.x * 32 + lane;
-    const int64_t share = (p.rows + p.parts - 1) / p.parts;
+    const int64_t share = (p.rows + p.sum_rows - 1) / p.sum_rows;
     const int64_t first = int64_t(blockIdx.y) * share, last = min(first + share, p.rows);
     float sum = 0.f;
     if (o < p.out)
@@ -32,7 +42,7 @@ __global__ void __launch_bounds__(kThreads) dy_sums_part(const __grid_constant__
 #pragma unroll
         for (int w = 1; w < kThreads / 32; ++w)
             sum += s_sum[w][lane];
-        p.partial[int64_t(blockIdx.y) * p.out + o] = sum;
+        p.sum_parts[int64_t(blockIdx.y) * p.out + o] = sum;
     }
 }
 
@@ -41,90 +51,390 @@ __global__ void __launch_bounds__(kThreads) dy_sums_join(const __grid_constant__
     if (o >= p.out)
         return;
     float sum = 0.f;
-    for (uint32_t part = 0; part < p.parts; ++part)
-        sum += p.partial[int64_t(part) * p.out + o];
+    for (uint32_t part = 0; part < p.sum_rows; ++part)
+        sum += p.sum_parts[int64_t(part) * p.out + o];
     p.dy_sums[o] = sum;
     if (p.dbias != nullptr)
         store_param(p.dbias, p.out_type, o, sum);
 }
 
-// 64 x 64 outputs per block, 16 rows at a time through shared memory.
+// ---------------------------------------------------------------- dy as bf16 terms
+// Each term is the rest's leading eight bits, cut (not rounded, which could
+// carry beyond bf16's range), so the rest is exact; a non-finite value is all
+// in the first.
 template <uint32_t TYPE>
-__global__ void __launch_bounds__(kThreads) weight_grad_any(const __grid_constant__ WeightGradParams p) {
-    __shared__ float s_dy[kDepth][kTile], s_x[kDepth][kTile];
-    const uint32_t o0 = blockIdx.y * kTile, k0 = blockIdx.x * kTile;
-    const uint32_t ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    float acc[4][4] = {};
-    for (int64_t m0 = 0; m0 < p.rows; m0 += kDepth) {
-        for (uint32_t i = threadIdx.x; i < kDepth * kTile; i += kThreads) {
-            const uint32_t d = i / kTile, c = i % kTile;
-            const int64_t m = m0 + d;
-            float a = 0.f, b = 0.f;
-            if (m < p.rows && o0 + c < p.out)
-                a = Element<TYPE>::get(static_cast<const typename Element<TYPE>::T *>(p.dy)[m * p.dy_stride + o0 + c]);
-            if (m < p.rows && k0 + c < p.width)
-                b = Element<kE4m3>::get(p.codes[m * p.codes_stride + k0 + c]) *
-                    p.scales[m * p.scale_row_stride + (k0 + c) / kCheckpointBlock * p.scale_col_stride];
-            s_dy[d][c] = a;
-            s_x[d][c] = b;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = s_dy[d][ty * 4 + i];
-                b[i] = s_x[d][tx * 4 + i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] += a[i] * b[j];
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t o = o0 + ty * 4 + i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t k = k0 + tx * 4 + j;
-            if (o >= p.out || k >= p.width)
-                continue;
-            float v = acc[i][j];
-            if (p.norm_weight != nullptr)
-                v *= load_param(p.norm_weight, p.param_type, k);
-            if (p.norm_bias != nullptr)
-                v += load_param(p.norm_bias, p.param_type, k) * p.dy_sums[o];
-            store_param(p.dweight, p.out_type, int64_t(o) * p.width + k, v);
+__global__ void __launch_bounds__(kThreads) split_dy(const __grid_constant__ WeightGradParams p) {
+    const int64_t total = p.rows * p.out, stride = int64_t(gridDim.x) * kThreads;
+    auto *planes = static_cast<uint16_t *>(p.dy_planes);
+    for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total; at += stride) {
+        const int64_t r = at / p.out;
+        const uint32_t o = uint32_t(at - r * p.out);
+        float rest = Element<TYPE>::get(static_cast<const typename Element<TYPE>::T *>(p.dy)[r * p.dy_stride + o]);
+        for (uint32_t plane = 0; plane < p.planes; ++plane) {
+            uint32_t bits = __float_as_uint(rest) & 0xFFFF0000u;
+            if (isnan(rest))
+                bits = 0x7FC00000u;
+            rest = fabsf(rest) <= FLT_MAX ? rest - __uint_as_float(bits) : 0.f;
+            planes[(int64_t(plane) * p.rows + r) * p.plane_stride + o] = uint16_t(bits >> 16);
         }
     }
 }
 
-template <uint32_t TYPE> void weight_grad(const WeightGradParams &p, cudaStream_t stream) {
+// ---------------------------------------------------------------- the product
+constexpr uint32_t kSteps = 64;              // rows per stage
+constexpr int kLoadStages = 3, kOperandStages = 2;
+constexpr uint32_t kDyChunk = kSteps * 128;  // 64 columns of dy (bf16)
+constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
+constexpr uint32_t kDyBytes = 4 * kDyChunk, kCodeBytes = 4 * kCodeChunk, kOperandBytes = 4 * kDyChunk;
+constexpr uint32_t kRingBytes = kLoadStages * (kDyBytes + kCodeBytes) + kOperandStages * kOperandBytes;
+constexpr uint32_t kSharedBytes = kRingBytes + 1024;  // + alignment of the swizzled tiles
+constexpr int kDecodeWarps = 8, kLoadWarp = 8, kMmaWarp = 9, kTensorThreads = 320;
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kStageRow = 66;           // floats per row of an epilogue tile
+constexpr uint64_t kWaitNs = 2000000000ull;  // far above any legal wait
+
+struct Shared {
+    uint64_t loaded[kLoadStages], load_free[kLoadStages];
+    uint64_t decoded[kOperandStages], operand_free[kOperandStages];
+    uint64_t done;
+    uint32_t tmem;
+    uint32_t failed;
+};
+
+__device__ __forceinline__ uint32_t to_bf16x2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Four codes as four bf16 values.
+__device__ __forceinline__ void decode4(uint32_t codes, float scale, uint32_t &low, uint32_t &high) {
+    const float2 a = from_e4m3x2(codes & 0xFFFFu), b = from_e4m3x2(codes >> 16);
+    low = to_bf16x2(a.x * scale, a.y * scale);
+    high = to_bf16x2(b.x * scale, b.y * scale);
+}
+
+// One block: halves x 128 outputs by tile_k columns over one part of the rows.
+// Warp 8 copies tiles of dy and codes into a ring of three stages; warps 0-7
+// decode a stage's codes into one of two operand buffers; warp 9 issues the
+// MMAs of a stage for both halves, so each decoded value is used 256 times.
+// Accumulators fill TMEM (2 x 256 columns).
+__global__ void __launch_bounds__(kTensorThreads, 1)
+    weight_grad_tensor(const __grid_constant__ WeightGradParams p, const __grid_constant__ CUtensorMap dy_map,
+                       const __grid_constant__ CUtensorMap code_map) {
+    extern __shared__ uint8_t s_raw[];
+    __shared__ Shared s;
+    uint8_t *ring = s_raw + ((1024u - (smem_addr(s_raw) & 1023u)) & 1023u);
+    uint8_t *dy_tiles = ring, *code_tiles = ring + kLoadStages * kDyBytes,
+            *operands = code_tiles + kLoadStages * kCodeBytes;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t o0 = blockIdx.x % p.tiles_o * (p.halves * 128);
+    const uint32_t k0 = blockIdx.x / p.tiles_o % p.tiles_k * p.tile_k;
+    const uint32_t part = blockIdx.x / (p.tiles_o * p.tiles_k);
+    const uint32_t plane_steps = uint32_t((p.rows + kSteps - 1) / kSteps);
+    const uint32_t first = part * p.part_steps;
+    const uint32_t steps = min(p.part_steps, plane_steps * p.planes - first);
+    const uint32_t columns = min(p.tile_k, p.width - k0);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kLoadStages; ++i) {
+            mbar_init(&s.loaded[i], 1);
+            mbar_init(&s.load_free[i], kDecodeWarps + 1);
+        }
+        for (int i = 0; i < kOperandStages; ++i) {
+            mbar_init(&s.decoded[i], kDecodeWarps);
+            mbar_init(&s.operand_free[i], 1);
+        }
+        mbar_init(&s.done, 1);
+        s.failed = 0;
+        fence_mbar_init();
+    }
+    if (warp == kMmaWarp)
+        tmem_alloc(&s.tmem, kTmemColumns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tmem = s.tmem;
+
+    bool ok = true;
+    if (warp == kLoadWarp) {
+        if (lane == 0) {
+            prefetch_tensor_map(&dy_map);
+            prefetch_tensor_map(&code_map);
+            const uint32_t dy_chunks = (min(p.halves * 128, p.out - o0) + 63) / 64, code_chunks = (columns + 63) / 64;
+            uint32_t i = 0;
+            for (; ok && i < steps; ++i) {
+                const uint32_t at = i % kLoadStages, g = first + i;
+                ok = mbar_wait(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
+                if (!ok)
+                    break;
+                const int m = int(g % plane_steps * kSteps), plane = int(g / plane_steps);
+                mbar_arrive_expect_tx(&s.loaded[at], dy_chunks * kDyChunk + code_chunks * kCodeChunk);
+                for (uint32_t c = 0; c < dy_chunks; ++c)
+                    tensor_load_3d(dy_tiles + at * kDyBytes + c * kDyChunk, &dy_map, int(o0 + c * 64), m, plane,
+                                   &s.loaded[at]);
+                for (uint32_t c = 0; c < code_chunks; ++c)
+                    tensor_load_3d(code_tiles + at * kCodeBytes + c * kCodeChunk, &code_map, int(k0 + c * 64), m, 0,
+                                   &s.loaded[at]);
+            }
+            if (!ok)  // let the copies in flight land before the block goes
+                for (uint32_t j = i > kLoadStages ? i - kLoadStages : 0; j < i; ++j)
+                    mbar_wait(&s.loaded[j % kLoadStages], j / kLoadStages & 1, kWaitNs);
+        }
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            const uint32_t shape = mma_shape_bf16(p.tile_k);
+            for (uint32_t i = 0; i < steps; ++i) {
+                const uint32_t at = i % kLoadStages, to = i % kOperandStages;
+                ok = mbar_wait(&s.loaded[at], i / kLoadStages & 1, kWaitNs) &&
+                     mbar_wait(&s.decoded[to], i / kOperandStages & 1, kWaitNs);
+                if (!ok)
+                    break;
+                tensor_fence_after();
+                for (uint32_t half = 0; half < p.halves; ++half)
+#pragma unroll
+                    for (uint32_t j = 0; j < kSteps / 16; ++j)
+                        mma_bf16(tmem + half * 256,
+                                 mma_operand(dy_tiles + at * kDyBytes + half * 2 * kDyChunk + j * 2048, kDyChunk, 1024),
+                                 mma_operand(operands + to * kOperandBytes + j * 2048, kDyChunk, 1024), shape,
+                                 (i | j) != 0);
+                mma_commit(&s.load_free[at]);
+                mma_commit(&s.operand_free[to]);
+            }
+            mma_commit(&s.done);
+        }
+    } else {
+        // A warp takes 32 rows and every fourth 16-byte unit of them: eight lanes
+        // of one shared-memory phase are eight rows of one unit, which both
+        // swizzles spread over all banks.
+        const uint32_t row = warp % 2 * 32 + lane, units = (columns + 15) / 16;
+        const uint32_t block0 = k0 / kCheckpointBlock;
+        const uint32_t blocks = (k0 + columns - 1) / kCheckpointBlock - block0 + 1;  // at most 3
+        const float *scales = p.scales + block0 * p.scale_col_stride;
+        float next[3];
+        auto load_scales = [&](uint32_t i) {
+            const int64_t m = int64_t((first + i) % plane_steps) * kSteps + row;
+#pragma unroll
+            for (uint32_t b = 0; b < 3; ++b)
+                next[b] = m < p.rows && b < blocks ? __ldg(scales + m * p.scale_row_stride + b * p.scale_col_stride) : 1.f;
+        };
+        load_scales(0);
+        for (uint32_t i = 0; i < steps; ++i) {
+            const uint32_t at = i % kLoadStages, to = i % kOperandStages;
+            const float scale0 = next[0], scale1 = next[1], scale2 = next[2];
+            if (i + 1 < steps)
+                load_scales(i + 1);
+            ok = mbar_wait(&s.loaded[at], i / kLoadStages & 1, kWaitNs) &&
+                 mbar_wait(&s.operand_free[to], (i / kOperandStages & 1) ^ 1, kWaitNs);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok)
+                break;
+            const uint8_t *codes = code_tiles + at * kCodeBytes + row * 64;
+            uint8_t *operand = operands + to * kOperandBytes + row * 128;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t u = warp / 2 + j * 4;
+                if (u < units) {
+                    const uint32_t b = (k0 + u * 16) / kCheckpointBlock - block0;
+                    const float scale = b == 0 ? scale0 : b == 1 ? scale1 : scale2;
+                    const Vec16 v = ld_shared_v4(codes + u / 4 * kCodeChunk + ((u % 4 ^ (row >> 1 & 3)) << 4));
+                    uint4 x, y;
+                    decode4(v.x, scale, x.x, x.y);
+                    decode4(v.y, scale, x.z, x.w);
+                    decode4(v.z, scale, y.x, y.y);
+                    decode4(v.w, scale, y.z, y.w);
+                    uint8_t *out = operand + u / 4 * kDyChunk;
+                    const uint32_t chunk = u % 4 * 2;
+                    *reinterpret_cast<uint4 *>(out + ((chunk ^ (row & 7)) << 4)) = x;
+                    *reinterpret_cast<uint4 *>(out + ((chunk + 1 ^ (row & 7)) << 4)) = y;
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&s.decoded[to]);
+                mbar_arrive(&s.load_free[at]);
+            }
+        }
+    }
+    if (!ok)
+        s.failed = 1;
+    __syncthreads();
+    if (warp < kDecodeWarps) {
+        ok = mbar_wait(&s.done, 0, kWaitNs);
+        ok = __all_sync(0xFFFFFFFFu, ok) && s.failed == 0;
+        tensor_fence_after();
+        if (ok) {
+            // A warp turns 32 rows x 64 columns at a time: TMEM lane = row, then
+            // rows of the tile in shared memory (the ring is free), then lane =
+            // column, so that rows are stored whole.
+            float *tile = reinterpret_cast<float *>(ring) + warp * 32 * kStageRow;
+            const uint32_t half = p.halves == 2 ? warp / 4 : 0, row0 = warp % 4 * 32;
+            const uint32_t chunk_step = p.halves == 2 ? 64 : 128;
+            const bool direct = p.parts == 1;
+            for (uint32_t c0 = p.halves == 2 ? 0 : warp / 4 * 64; c0 < columns; c0 += chunk_step) {
+                uint32_t v[2][32];
+                const uint32_t address = tmem + (row0 << 16) + half * 256 + c0;
+                tmem_load32(address, v[0]);
+                if (c0 + 32 < columns)
+                    tmem_load32(address + 32, v[1]);
+                tmem_wait_loads();
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    tile[lane * kStageRow + c] = __uint_as_float(v[c / 32][c % 32]);
+                __syncwarp();
+                const uint32_t c = c0 + lane * 2, k = k0 + c;
+                const bool there[2] = {c < columns, c + 1 < columns};
+                float w[2] = {1.f, 1.f}, b[2] = {0.f, 0.f};
+                for (int e = 0; e < 2; ++e)
+                    if (direct && there[e]) {
+                        if (p.norm_weight != nullptr)
+                            w[e] = load_param(p.norm_weight, p.param_type, k + e);
+                        if (p.norm_bias != nullptr)
+                            b[e] = load_param(p.norm_bias, p.param_type, k + e);
+                    }
+                for (uint32_t r = 0; r < 32; ++r) {
+                    const uint32_t o = o0 + half * 128 + row0 + r;
+                    if (o >= p.out)
+                        break;
+                    float2 x = *reinterpret_cast<const float2 *>(tile + r * kStageRow + lane * 2);
+                    const int64_t at = int64_t(o) * p.width + k;
+                    if (!direct) {
+                        float *to = p.dw_parts + int64_t(part) * p.out * p.width + at;
+                        if (there[0])
+                            to[0] = x.x;
+                        if (there[1])
+                            to[1] = x.y;
+                        continue;
+                    }
+                    if (p.norm_weight != nullptr) {
+                        x.x *= w[0];
+                        x.y *= w[1];
+                    }
+                    if (p.norm_bias != nullptr) {
+                        const float sum = p.dy_sums[o];
+                        x.x += b[0] * sum;
+                        x.y += b[1] * sum;
+                    }
+                    if (there[1] && p.out_type == kBf16 && p.width % 2 == 0) {
+                        reinterpret_cast<uint32_t *>(p.dweight)[at / 2] = to_bf16x2(x.x, x.y);
+                        continue;
+                    }
+                    if (there[0])
+                        store_param(p.dweight, p.out_type, at, x.x);
+                    if (there[1])
+                        store_param(p.dweight, p.out_type, at + 1, x.y);
+                }
+            }
+        }
+        tensor_fence_before();
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tensor_fence_after();
+        tmem_free(tmem, kTmemColumns);
+        if (lane == 0 && s.failed != 0)
+            st_release_sys_u32(p.fault, kPipelineTimeout);
+    }
+    if (warp < kDecodeWarps && !ok && lane == 0)
+        st_release_sys_u32(p.fault, kPipelineTimeout);
+}
+
+// Adds the parts of the rows in order, and folds the norm in.
+__global__ void __launch_bounds__(kThreads) weight_grad_join(const __grid_constant__ WeightGradParams p) {
+    const int64_t total = int64_t(p.out) * p.width, stride = int64_t(gridDim.x) * kThreads;
+    for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total; at += stride) {
+        float v = 0.f;
+        for (uint32_t part = 0; part < p.parts; ++part)
+            v += p.dw_parts[part * total + at];
+        const int64_t o = at / p.width;
+        const uint32_t k = uint32_t(at - o * p.width);
+        if (p.norm_weight != nullptr)
+            v *= load_param(p.norm_weight, p.param_type, k);
+        if (p.norm_bias != nullptr)
+            v += load_param(p.norm_bias, p.param_type, k) * p.dy_sums[o];
+        store_param(p.dweight, p.out_type, at, v);
+    }
+}
+
+// [planes][rows][columns] with boxes of 64 rows x 64 columns; what lies outside reads as zero.
+CUtensorMap tile_map(CUtensorMapDataType type, const void *base, uint64_t columns, uint64_t rows,
+                     uint64_t planes, uint64_t row_bytes, CUtensorMapSwizzle swizzle) {
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {columns, rows, planes}, strides[2] = {row_bytes, row_bytes * rows};
+    const cuuint32_t box[3] = {64, kSteps, 1}, steps[3] = {1, 1, 1};
+    check_cu(driver().TensorMapEncodeTiled(&map, type, 3, const_cast<void *>(base), dims, strides, box, steps,
+                                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+             "encode tensor map");
+    return map;
+}
+
+template <uint32_t TYPE> void dy_passes(const WeightGradParams &p, cudaStream_t stream) {
     if (p.dy_sums != nullptr) {
-        dy_sums_part<TYPE><<<dim3((p.out + 31) / 32, p.parts), kThreads, 0, stream>>>(p);
+        dy_sums_part<TYPE><<<dim3((p.out + 31) / 32, p.sum_rows), kThreads, 0, stream>>>(p);
         dy_sums_join<<<(p.out + kThreads - 1) / kThreads, kThreads, 0, stream>>>(p);
     }
-    weight_grad_any<TYPE><<<dim3((p.width + kTile - 1) / kTile, (p.out + kTile - 1) / kTile), kThreads, 0, stream>>>(p);
+    if (p.planes > 1)
+        split_dy<TYPE><<<uint32_t(std::min<int64_t>((p.rows * p.out + kThreads - 1) / kThreads, 148 * 16)), kThreads, 0,
+                         stream>>>(p);
 }
 
 } // namespace
 
-uint32_t weight_grad_parts(const WeightGradParams &p, int num_sms) {
+void plan_weight_grad(WeightGradParams &p, int num_sms) {
     const int64_t want = int64_t(num_sms) * 4 * 32 / p.out + 1, most = (p.rows + 31) / 32;
-    return uint32_t(want < most ? want : most);
+    p.sum_rows = uint32_t(std::min(want, most));
+    p.planes = p.type == kBf16 ? 1 : p.type == kFp16 ? 2 : 3;
+    p.halves = p.out > 128 ? 2 : 1;
+    p.tiles_o = (p.out + p.halves * 128 - 1) / (p.halves * 128);
+    const int64_t steps = (p.rows + kSteps - 1) / kSteps * p.planes;
+    // Cycles of one block: a stage is bound by its MMAs (128 x 16 x n takes n / 2)
+    // or its decoding (about 20 values a cycle); the epilogue moves ~12 values a
+    // cycle.  Splitting the rows costs a pass over the parts at ~3.5 KB a cycle.
+    double best = 1e300;
+    for (uint32_t tile = 16; tile <= 256; tile += 16) {
+        const uint32_t tiles_k = (p.width + tile - 1) / tile;
+        const int64_t tiles = int64_t(p.tiles_o) * tiles_k;
+        for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 64); parts = parts < 8 ? parts + 1 : parts * 2) {
+            const int64_t part_steps = (steps + parts - 1) / parts, used = (steps + part_steps - 1) / part_steps;
+            const double waves = double((tiles * used + num_sms - 1) / num_sms);
+            const double stage = std::max(2.0 * p.halves * tile, 64.0 * tile / 20 + 150);
+            const double block = 3000 + part_steps * stage + p.halves * 128.0 * tile / 12;
+            const double join = used > 1 ? 3000 + 8.0 * used * p.out * p.width / 3500 : 0;
+            const double cost = waves * block + join;
+            if (cost < best * 0.999) {
+                best = cost;
+                p.tile_k = tile;
+                p.tiles_k = tiles_k;
+                p.parts = uint32_t(used);
+                p.part_steps = uint32_t(part_steps);
+            }
+        }
+    }
 }
 
-cudaError_t launch_weight_grad(const WeightGradParams &p, int, cudaStream_t stream) {
+cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
     if (p.type == kBf16)
-        weight_grad<kBf16>(p, stream);
+        dy_passes<kBf16>(p, stream);
     else if (p.type == kFp16)
-        weight_grad<kFp16>(p, stream);
+        dy_passes<kFp16>(p, stream);
     else
-        weight_grad<kFp32>(p, stream);
+        dy_passes<kFp32>(p, stream);
+    const bool split = p.planes > 1;
+    const CUtensorMap dy_map =
+        tile_map(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, split ? p.dy_planes : p.dy, p.out, p.rows, p.planes,
+                 uint64_t(split ? p.plane_stride : p.dy_stride) * 2, CU_TENSOR_MAP_SWIZZLE_128B);
+    const CUtensorMap code_map = tile_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, p.codes, p.width, p.rows, 1,
+                                          uint64_t(p.codes_stride), CU_TENSOR_MAP_SWIZZLE_64B);
+    cudaError_t rc = cudaFuncSetAttribute(weight_grad_tensor, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    if (rc != cudaSuccess)
+        return rc;
+    weight_grad_tensor<<<p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(p, dy_map, code_map);
+    if (p.parts > 1) {
+        const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
+        weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(p);
+    }
     return cudaGetLastError();
 }
 

@@ -41,6 +41,7 @@ const DriverApi &driver() {
         load("cuMemGetAllocationGranularity", api.MemGetAllocationGranularity);
         load("cuDeviceGetAttribute", api.DeviceGetAttribute);
         load("cuGetErrorString", api.GetErrorString);
+        load("cuTensorMapEncodeTiled", api.TensorMapEncodeTiled);
     });
     if (!failure.empty())
         throw std::runtime_error(failure);

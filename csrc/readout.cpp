@@ -8,8 +8,10 @@
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
+#include <array>
+#include <cstring>
+#include <mutex>
 #include <optional>
-#include <string>
 
 #include "bindings.h"
 #include "driver.h"
@@ -87,6 +89,39 @@ Tensor empty_codes(const Tensor &like, int64_t rows, int64_t width) {
 
 Tensor empty_scales(const Tensor &like, int64_t rows, int64_t width) {
     return at::empty({rows, (width + kCheckpointBlock - 1) / kCheckpointBlock}, like.options().dtype(ScalarType::Float));
+}
+
+// Rows that start on 16-byte boundaries, one after the other.
+bool on_16_bytes(const Tensor &t, int64_t size) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) * size % 16 == 0 &&
+           t.stride(0) >= t.size(1);
+}
+
+// One host-mapped word per device that a kernel sets when one of its bounded
+// waits ran out (its results are then not to be used); it is read before every
+// launch without synchronising.
+uint32_t *fault_word(int device) {
+    static std::mutex mutex;
+    static std::array<uint32_t *, 64> words{};
+    check(device >= 0 && device < int(words.size()), "device index out of range");
+    std::lock_guard<std::mutex> lock(mutex);
+    if (words[device] == nullptr) {
+        // Allowed while a graph is captured: the allocation is no part of it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+        void *word = nullptr;
+        const cudaError_t rc = cudaHostAlloc(&word, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        check_cuda(rc, "allocate fault word");
+        std::memset(word, 0, 64);
+        words[device] = static_cast<uint32_t *>(word);
+    }
+    return words[device];
+}
+
+void need_healthy(const uint32_t *fault) {
+    check(*static_cast<const volatile uint32_t *>(fault) == 0,
+          "an earlier weight gradient on this GPU gave up waiting for its pipeline; its results are invalid");
 }
 
 // (y, codes | None, scales | None, mean | None, rstd | None)
@@ -294,9 +329,9 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     const OptTensor codes_opt = codes, scales_opt = scales;
     const int device = need_device(dy, {&codes_opt, &scales_opt, &norm_weight, &norm_bias});
     c10::cuda::CUDAGuard guard(device);
-    const auto options = dy.options().dtype(result);
+    const auto options = dy.options().dtype(result), floats = dy.options().dtype(ScalarType::Float);
     const Tensor dweight = at::empty({out, width}, options);
-    OptTensor dbias, sums, partial;
+    OptTensor dbias, sums;
     if (want_bias)
         dbias = at::empty({out}, options);
     if (rows == 0) {
@@ -305,17 +340,30 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
             dbias->zero_();
         return py::make_tuple(dweight, dbias);
     }
+    uint32_t *fault = fault_word(device);
+    need_healthy(fault);
+    // Tiled copies want rows on 16-byte boundaries; others are copied first.
+    Tensor rows_dy = dy, rows_codes = codes;
+    if (dy.scalar_type() == ScalarType::BFloat16 && !on_16_bytes(dy, 2)) {
+        rows_dy = at::empty({rows, (out + 7) / 8 * 8}, dy.options()).narrow(1, 0, out);
+        rows_dy.copy_(dy);
+    }
+    if (!on_16_bytes(codes, 1)) {
+        rows_codes = empty_codes(codes, rows, width);
+        rows_codes.copy_(codes);
+    }
     WeightGradParams p{};
-    p.dy = dy.data_ptr();
-    p.codes = static_cast<const uint8_t *>(codes.data_ptr());
+    p.dy = rows_dy.data_ptr();
+    p.codes = static_cast<const uint8_t *>(rows_codes.data_ptr());
     p.scales = static_cast<const float *>(scales.data_ptr());
     p.norm_weight = data(norm_weight);
     p.norm_bias = data(norm_bias);
     p.dweight = dweight.data_ptr();
     p.dbias = data(dbias);
+    p.fault = fault;
     p.rows = rows;
-    p.dy_stride = dy.stride(0);
-    p.codes_stride = codes.stride(0);
+    p.dy_stride = rows_dy.stride(0);
+    p.codes_stride = rows_codes.stride(0);
     p.scale_row_stride = scales.stride(0);
     p.scale_col_stride = scales.stride(1);
     p.width = uint32_t(width);
@@ -323,15 +371,23 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     p.type = element_type(dy.scalar_type());
     p.param_type = norm_weight ? element_type(norm_weight->scalar_type()) : 0;
     p.out_type = element_type(result);
-    const int sms = sm_count(device);
+    plan_weight_grad(p, sm_count(device));
+    OptTensor planes, dw_parts;
     if (want_bias || norm_bias) {
-        p.parts = weight_grad_parts(p, sms);
-        sums = at::empty({out}, dy.options().dtype(ScalarType::Float));
-        partial = at::empty({int64_t(p.parts), out}, dy.options().dtype(ScalarType::Float));
+        sums = at::empty({int64_t(p.sum_rows) + 1, out}, floats);
         p.dy_sums = static_cast<float *>(sums->data_ptr());
-        p.partial = static_cast<float *>(partial->data_ptr());
+        p.sum_parts = p.dy_sums + out;
     }
-    check_cuda(launch_weight_grad(p, sms, at::cuda::getCurrentCUDAStream(device).stream()), "launch weight gradient");
+    if (p.planes > 1) {
+        p.plane_stride = (out + 7) / 8 * 8;
+        planes = at::empty({int64_t(p.planes), rows, p.plane_stride}, dy.options().dtype(ScalarType::BFloat16));
+        p.dy_planes = planes->data_ptr();
+    }
+    if (p.parts > 1) {
+        dw_parts = at::empty({int64_t(p.parts), out, width}, floats);
+        p.dw_parts = static_cast<float *>(dw_parts->data_ptr());
+    }
+    check_cuda(launch_weight_grad(p, at::cuda::getCurrentCUDAStream(device).stream()), "launch weight gradient");
     return py::make_tuple(dweight, dbias);
 }
 
