@@ -101,11 +101,6 @@ struct Shared {
     uint32_t failed;
 };
 
-__device__ __forceinline__ uint32_t to_bf16x2(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-
 // Four codes as four bf16 values.
 __device__ __forceinline__ void decode4(uint32_t codes, float scale, uint32_t &low, uint32_t &high) {
     const float2 a = from_e4m3x2(codes & 0xFFFFu), b = from_e4m3x2(codes >> 16);
