@@ -43,7 +43,10 @@ template <> struct RowReader<kE4m3> {
 // times (twice from cache).
 template <uint32_t IN, uint32_t OUT>
 __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_constant__ NormForwardParams p) {
-    __shared__ float2 s_sum[2][kRowWarps];
+    __shared__ WarpSums s_sum[2];
+    clear_sums(s_sum[0]);
+    clear_sums(s_sum[1]);
+    __syncthreads();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const float inv = 1.f / float(p.width);
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -51,7 +54,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
         float a = 0.f, b = 0.f;
         for (uint32_t c = threadIdx.x; c < p.width; c += kRowThreads)
             a += x(c);
-        float mean = block_sum2(a, 0.f, s_sum[0]).x * inv;
+        float mean = block_sum(a, s_sum[0]) * inv;
         a = 0.f;
         for (uint32_t c = threadIdx.x; c < p.width; c += kRowThreads) {
             const float d = x(c) - mean;
@@ -104,115 +107,174 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
     }
 }
 
-// A row of whole 8-value chunks on vector boundaries, held in registers: one
-// pass over memory.  Chunk c of a row is thread c % T's, T the block (or, for
-// rows of at most 32 V chunks, each warp, which then has a row of its own).
-// Sixteen lanes hold a checkpoint block, so its largest value takes four
-// shuffles.
-template <uint32_t IN, uint32_t OUT, int V>
-__global__ void __launch_bounds__(1024) norm_forward_row(const __grid_constant__ NormForwardParams p, bool warp_rows) {
-    __shared__ float2 s_sum[2][32];
-    const uint32_t lane = threadIdx.x % 32, chunks = p.width / 8;
-    const uint32_t t = warp_rows ? lane : threadIdx.x, stride = warp_rows ? 32 : blockDim.x;
-    const int64_t r = warp_rows ? int64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : int64_t(blockIdx.x);
-    if (r >= p.rows)
-        return;  // a whole warp of a block of warp rows
+// Rows of whole 8-value chunks on vector boundaries.  A warp holds 32 V adjacent
+// chunks of its row, lane l those with l = c % 32, so all of a thread's offsets
+// are constants; FULL: every thread has V of them.  A row takes a block of
+// warps or, with at most 32 V chunks, one warp of a block.  Blocks stay and
+// take every gridDim-th row (warp row).  What a thread needs of the rows to
+// come it copies itself into its own slots of shared memory, slot_depth - 1
+// rows ahead, so no barrier guards the copies and they cost no registers.
+constexpr int slot_depth(uint32_t type) { return type == kFp32 ? 2 : 3; }
+
+struct RowShare {
+    uint32_t row, step, chunk;  // first row, rows to the next, first chunk
+    __device__ __forceinline__ RowShare(bool warp_rows, int vectors) {
+        const uint32_t warp = threadIdx.x / 32, warps = blockDim.x / 32;
+        row = warp_rows ? blockIdx.x * warps + warp : blockIdx.x;
+        step = warp_rows ? gridDim.x * warps : gridDim.x;
+        chunk = threadIdx.x % 32 + (warp_rows ? 0 : warp * 32 * vectors);
+    }
+};
+
+// A warp's bytes of one depth of slots: V x 32 chunks, then their scales.
+template <uint32_t IN, int V> struct ForwardSlots {
+    static constexpr int kDepth = slot_depth(IN);
+    static constexpr uint32_t kChunk = 32 * Raw8<IN>::kBytes;
+    static constexpr uint32_t kScales = V * kChunk;
+    static constexpr uint32_t kDepthBytes = kScales + (IN == kE4m3 ? V * 128 : 0);
+};
+
+// The row is read once and held in registers between the two sums and the
+// output.  Sixteen lanes hold a checkpoint block, so its largest value takes
+// four shuffles.
+template <uint32_t IN, uint32_t OUT, uint32_t PARAM, int V, bool FULL, bool FP8, int T>
+__global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
+    norm_forward_row(const __grid_constant__ NormForwardParams p, bool warp_rows) {
+    using Slots = ForwardSlots<IN, V>;
+    extern __shared__ __align__(16) uint8_t s_slots[];
+    __shared__ WarpSums s_sum[2];
+    clear_sums(s_sum[0]);
+    clear_sums(s_sum[1]);
+    __syncthreads();
+    const RowShare share(warp_rows, V);
+    const uint32_t chunks = p.width / 8, rows = uint32_t(p.rows), lane = threadIdx.x % 32;
     const float inv = 1.f / float(p.width);
-    const uint8_t *row = static_cast<const uint8_t *>(p.x) + r * p.x_stride * int64_t(sizeof(typename Element<IN>::T));
-    float x[V][8];
-    Raw8<IN> raw[V];
-    float scale[V];
+    const uint32_t warp_slots = smem_addr(s_slots) + threadIdx.x / 32 * (Slots::kDepthBytes * Slots::kDepth);
+    const uint32_t x_slot = warp_slots + lane * (IN == kE4m3 ? 8 : 16), scale_slot = warp_slots + Slots::kScales + lane * 4;
+    const auto there = [&](int i) { return FULL || share.chunk + i * 32 < chunks; };
+
+    const uint8_t *x_at = static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(IN)) +
+                          share.chunk * Raw8<IN>::kBytes;
+    const int64_t x_step = share.step * p.x_stride * int64_t(element_bytes(IN));
+    const float *scale_at = IN == kE4m3 ? p.scales + share.row * p.scale_row_stride : nullptr;
+    uint32_t pack[V];
+    if constexpr (IN == kE4m3) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const uint32_t c = t + i * stride;
-        scale[i] = 1.f;
-        if (c < chunks) {
-            raw[i] = load_row8<IN>(row + c * Raw8<IN>::kBytes);
-            if constexpr (IN == kE4m3) {
-                const uint32_t entry = c * 8 / p.hidden, column = c * 8 - entry * p.hidden;
-                scale[i] = __ldg(p.scales + r * p.scale_row_stride +
-                                 (entry * p.packs + column / p.block) * p.scale_col_stride);
-            }
+        for (int i = 0; i < V; ++i) {
+            const uint32_t column = (share.chunk + i * 32) * 8, entry = column / p.hidden;
+            pack[i] = entry * p.packs + (column - entry * p.hidden) / p.block;
         }
     }
-    float a = 0.f, b = 0.f;
+    uint32_t copied = share.row;
+    auto copy = [&](uint32_t depth) {
+        if (copied < rows) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if (t + i * stride < chunks) {
-            unpack8<IN>(raw[i], x[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (IN == kE4m3)
-                    x[i][e] *= scale[i];
-                a += x[i][e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[i][e] = 0.f;
+            for (int i = 0; i < V; ++i)
+                if (there(i)) {
+                    copy_shared8<IN>(x_slot + depth + i * Slots::kChunk, 512, x_at + i * 32 * Raw8<IN>::kBytes);
+                    if constexpr (IN == kE4m3)
+                        copy_shared4(scale_slot + depth + i * 128, scale_at + pack[i] * p.scale_col_stride);
+                }
+            x_at += x_step;
+            if constexpr (IN == kE4m3)
+                scale_at += share.step * p.scale_row_stride;
         }
-    }
-    float mean = (warp_rows ? lanes_sum2(a, 0.f) : block_sum2(a, 0.f, s_sum[0])).x * inv;
-    a = 0.f;
+        copied += share.step;
+        cp_async_commit();
+    };
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (t + i * stride < chunks) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float d = x[i][e] - mean;
-                a += d;
-                b += d * d;
-            }
-        }
-    const float2 sums = warp_rows ? lanes_sum2(a, b) : block_sum2(a, b, s_sum[1]);
-    const float shift = sums.x * inv;
-    const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
-    mean += shift;
-    if (t == 0) {
-        if (p.keep == kKeepStats)
-            p.mean[r] = mean;
-        if (p.keep != kKeepNothing)
-            p.rstd[r] = rstd;
-    }
-    uint8_t *y = static_cast<uint8_t *>(p.y) + r * p.width * int64_t(sizeof(typename Element<OUT>::T));
+    for (int d = 0; d < Slots::kDepth - 1; ++d)
+        copy(d * Slots::kDepthBytes);
+    uint32_t slot = 0, refill = (Slots::kDepth - 1) * Slots::kDepthBytes;
+    uint8_t *y_at = static_cast<uint8_t *>(p.y) + int64_t(share.row) * p.width * element_bytes(OUT) + share.chunk * Raw8<OUT>::kBytes;
+    const int64_t y_step = int64_t(share.step) * p.width * element_bytes(OUT);
+    const uint8_t *w_at = static_cast<const uint8_t *>(p.weight) + share.chunk * Raw8<PARAM>::kBytes;
+    const uint8_t *b_at = static_cast<const uint8_t *>(p.bias) + share.chunk * Raw8<PARAM>::kBytes;
     const uint32_t blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
+    const bool affine = p.weight != nullptr, shifted = p.bias != nullptr;
+    for (uint32_t r = share.row; r < rows; r += share.step) {
+        cp_async_wait<Slots::kDepth - 2>();
+        Pair x[V][4];
+        Pair a = both(0.f), b = both(0.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const uint32_t c = t + i * stride;
-        const bool there = c < chunks;
-        float amax = 0.f;
-        if (there) {
-            float v[8];
+        for (int i = 0; i < V; ++i)
+            if (there(i)) {
+                load_shared8<IN>(x_slot + slot + i * Slots::kChunk, 512, x[i]);
+                if constexpr (IN == kE4m3) {
+                    const Pair scale = both(load_shared1(scale_slot + slot + i * 128));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[i][e] = (x[i][e] - mean) * rstd;
-                amax = fmaxf(amax, finite_abs(x[i][e]));
-                v[e] = x[i][e];
+                    for (int e = 0; e < 4; ++e)
+                        x[i][e] = mul2(x[i][e], scale);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    a = add2(a, x[i][e]);
             }
-            if (p.weight != nullptr) {
-                float w[8];
-                load_param8(p.weight, p.param_type, c * 8, w);
+        copy(refill);  // the row before this one was there, and this thread alone read it
+        refill = slot;
+        slot = slot + Slots::kDepthBytes == Slots::kDepth * Slots::kDepthBytes ? 0 : slot + Slots::kDepthBytes;
+        const float mean = (warp_rows ? lanes_sum(total(a)) : block_sum(total(a), s_sum[0])) * inv;
+        const Pair minus_mean = both(-mean);
+        a = both(0.f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] *= w[e];
-            }
-            if (p.bias != nullptr) {
-                float w[8];
-                load_param8(p.bias, p.param_type, c * 8, w);
+        for (int i = 0; i < V; ++i)
+            if (there(i)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] += w[e];
+                for (int e = 0; e < 4; ++e) {
+                    x[i][e] = add2(x[i][e], minus_mean);
+                    a = add2(a, x[i][e]);
+                    b = fma2(x[i][e], x[i][e], b);
+                }
             }
-            store_row8<OUT>(y + c * Raw8<OUT>::kBytes, v);
+        const float2 sums = warp_rows ? lanes_sum2(total(a), total(b)) : block_sum2(total(a), total(b), s_sum[1]);
+        const float shift = sums.x * inv;
+        const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
+        if (share.chunk == 0 && p.keep != kKeepNothing) {
+            if (p.keep == kKeepStats)
+                p.mean[r] = mean + shift;
+            p.rstd[r] = rstd;
         }
-        if (p.keep == kKeepFp8) {
-            const int k = block_exponent(lanes_max<16>(amax));
-            if (there) {
-                *reinterpret_cast<uint2 *>(p.codes + r * p.codes_stride + c * 8) = to_e4m3x8(x[i], exp2_int(-k));
-                if (lane % 16 == 0)
-                    p.code_scales[r * blocks + c / 16] = exp2_int(k);
+        const Pair minus_shift = both(-shift), up = both(rstd);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float amax = 0.f;
+            if (there(i)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // Finite, or NaN in all of a row: an infinity makes the mean NaN or infinite.
+                    x[i][e] = mul2(add2(x[i][e], minus_shift), up);
+                    if constexpr (FP8)
+                        amax = fmaxf(amax, fmaxf(fabsf(parts(x[i][e]).x), fabsf(parts(x[i][e]).y)));
+                }
+                if (affine) {
+                    Pair v[4], w[4];
+                    load_param8<PARAM>(w_at + i * 32 * Raw8<PARAM>::kBytes, w);
+                    if (shifted) {
+                        load_param8<PARAM>(b_at + i * 32 * Raw8<PARAM>::kBytes, v);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = fma2(x[i][e], w[e], v[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = mul2(x[i][e], w[e]);
+                    }
+                    store_row8<OUT>(y_at + i * 32 * Raw8<OUT>::kBytes, v);
+                } else {
+                    store_row8<OUT>(y_at + i * 32 * Raw8<OUT>::kBytes, x[i]);
+                }
+            }
+            if constexpr (FP8) {
+                const int k = block_exponent(lanes_max<16>(amax));
+                if (there(i)) {
+                    const uint32_t c = share.chunk + i * 32;
+                    *reinterpret_cast<uint2 *>(p.codes + r * p.codes_stride + c * 8) = to_e4m3x8(x[i], exp2_int(-k));
+                    if (lane % 16 == 0)
+                        p.code_scales[int64_t(r) * blocks + c / 16] = exp2_int(k);
+                }
             }
         }
+        y_at += y_step;
     }
 }
 
@@ -228,7 +290,10 @@ template <uint32_t X> __device__ __forceinline__ float kept_value(const NormBack
 
 template <uint32_t X, uint32_t DY>
 __global__ void __launch_bounds__(kRowThreads) norm_backward_rows_any(const __grid_constant__ NormBackwardParams p) {
-    __shared__ float2 s_sum[2][kRowWarps];
+    __shared__ WarpSums s_sum[2];
+    clear_sums(s_sum[0]);
+    clear_sums(s_sum[1]);
+    __syncthreads();
     const float inv = 1.f / float(p.width);
     uint32_t turn = 0;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
@@ -306,153 +371,139 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
 }
 
 // Rows of whole chunks (as in norm_forward_row), dx and the column sums in one
-// pass over memory.  A block stays and takes every gridDim-th row (or warp
-// row), so a thread owns the same columns in all of them: its sums for dweight
-// and dbias stay in registers, and each block leaves one part of them.  What a
-// thread needs of the rows to come it copies itself into its own slots of
-// shared memory, DEPTH - 1 rows ahead, so no barrier guards the copies.
+// pass over memory.  A thread owns the same columns in all rows of its block:
+// its sums for dweight and dbias stay in registers, and each block leaves one
+// part of them.  Its slots: dy's chunks, the kept rows' chunks, their scales.
 template <uint32_t X, uint32_t DY, int V> struct BackwardSlots {
-    static constexpr int kDepth = DY == kFp32 ? 2 : 3;
-    static constexpr int kChunk = Raw8<DY>::kBytes + Raw8<X>::kBytes + (X == kE4m3 ? 4 : 0);  // bytes per thread
-    static constexpr int kThread = kDepth * V * kChunk;
+    static constexpr int kDepth = slot_depth(DY);
+    static constexpr uint32_t kDyChunk = 32 * Raw8<DY>::kBytes, kXChunk = 32 * Raw8<X>::kBytes;
+    static constexpr uint32_t kX = V * kDyChunk, kScales = kX + V * kXChunk;
+    static constexpr uint32_t kDepthBytes = kScales + (X == kE4m3 ? V * 128 : 0);
 };
 
-template <uint32_t TYPE> __device__ __forceinline__ void copy_row8(void *slot, uint32_t slot_stride, const uint8_t *src) {
-    if constexpr (TYPE == kE4m3) {
-        cp_async_8(slot, src);
-    } else {
-        cp_async_16(slot, src);
-        if constexpr (TYPE == kFp32)
-            cp_async_16(static_cast<uint8_t *>(slot) + slot_stride, src + 16);
-    }
-}
-
-template <uint32_t TYPE> __device__ __forceinline__ void slot_row8(const void *slot, uint32_t slot_stride, float (&x)[8]) {
-    Raw8<TYPE> r;
-    if constexpr (TYPE == kE4m3) {
-        r.v = *static_cast<const uint2 *>(slot);
-    } else {
-        r.v = ld_shared_v4(slot);
-        if constexpr (TYPE == kFp32)
-            r.v2 = ld_shared_v4(static_cast<const uint8_t *>(slot) + slot_stride);
-    }
-    unpack8<TYPE>(r, x);
-}
-
-template <uint32_t X, uint32_t DY, int V>
-__global__ void __launch_bounds__(512) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
+template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
+__global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
     using Slots = BackwardSlots<X, DY, V>;
-    constexpr int kDepth = Slots::kDepth;
     extern __shared__ __align__(16) uint8_t s_slots[];
-    __shared__ float2 s_sum[2][16];
-    const uint32_t lane = threadIdx.x % 32, threads = blockDim.x, chunks = p.width / 8;
-    const uint32_t t = warp_rows ? lane : threadIdx.x, stride = warp_rows ? 32 : threads;
-    const int64_t first = warp_rows ? int64_t(blockIdx.x) * (threads / 32) + threadIdx.x / 32 : int64_t(blockIdx.x);
-    const int64_t step = warp_rows ? int64_t(gridDim.x) * (threads / 32) : int64_t(gridDim.x);
+    __shared__ WarpSums s_sum[2];
+    clear_sums(s_sum[0]);
+    clear_sums(s_sum[1]);
+    const RowShare share(warp_rows, V);
+    const uint32_t chunks = p.width / 8, rows = uint32_t(p.rows), lane = threadIdx.x % 32;
     const float inv = 1.f / float(p.width);
-    // Slots: per depth and chunk, 16-byte (codes: 8) pieces side by side over the
-    // threads, then the scales.
-    const uint32_t piece = threads * 16;
-    uint8_t *dy_slots = s_slots, *x_slots = dy_slots + kDepth * V * threads * Raw8<DY>::kBytes;
-    float *scale_slots = reinterpret_cast<float *>(x_slots + kDepth * V * threads * Raw8<X>::kBytes);
-    auto dy_slot = [&](int d, int i) { return dy_slots + (d * V + i) * threads * Raw8<DY>::kBytes + threadIdx.x * 16; };
-    auto x_slot = [&](int d, int i) {
-        return x_slots + (d * V + i) * threads * Raw8<X>::kBytes + threadIdx.x * (X == kE4m3 ? 8 : 16);
-    };
-    auto scale_slot = [&](int d, int i) { return scale_slots + (d * V + i) * threads + threadIdx.x; };
+    const uint32_t warp_bytes = Slots::kDepthBytes * Slots::kDepth;
+    const uint32_t warp_slots = smem_addr(s_slots) + threadIdx.x / 32 * warp_bytes;
+    const uint32_t dy_slot = warp_slots + lane * 16, x_slot = warp_slots + Slots::kX + lane * (X == kE4m3 ? 8 : 16);
+    const uint32_t scale_slot = warp_slots + Slots::kScales + lane * 4;
+    const auto there = [&](int i) { return share.chunk + i * 32 < chunks; };
+    // What no chunk fills is zero, so that it adds nothing.
+    for (uint32_t at = threadIdx.x * 4; at < warp_bytes * (blockDim.x / 32); at += blockDim.x * 4)
+        *reinterpret_cast<uint32_t *>(s_slots + at) = 0;
+    __syncthreads();
 
-    auto copy = [&](int64_t r, int d) {
-        if (r < p.rows) {
-            const uint8_t *dy = static_cast<const uint8_t *>(p.dy) + r * p.dy_stride * int64_t(element_bytes(DY));
-            const uint8_t *x = X == kE4m3 ? p.codes + r * p.codes_stride
-                                          : static_cast<const uint8_t *>(p.x) + r * p.x_stride * int64_t(element_bytes(X));
+    const uint8_t *dy_at = static_cast<const uint8_t *>(p.dy) + share.row * p.dy_stride * int64_t(element_bytes(DY)) +
+                           share.chunk * Raw8<DY>::kBytes;
+    const uint8_t *x_at = X == kE4m3 ? p.codes + share.row * p.codes_stride
+                                     : static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(X));
+    x_at += share.chunk * Raw8<X>::kBytes;
+    const float *scale_at =
+        X == kE4m3 ? p.code_scales + share.row * p.code_scales_stride + share.chunk / 16 * p.scale_col_stride : nullptr;
+    const int64_t dy_step = share.step * p.dy_stride * int64_t(element_bytes(DY));
+    const int64_t x_step = X == kE4m3 ? share.step * p.codes_stride : share.step * p.x_stride * int64_t(element_bytes(X));
+    uint32_t copied = share.row;
+    auto copy = [&](uint32_t depth) {
+        if (copied < rows) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const uint32_t c = t + i * stride;
-                if (c < chunks) {
-                    copy_row8<DY>(dy_slot(d, i), piece, dy + c * Raw8<DY>::kBytes);
-                    copy_row8<X>(x_slot(d, i), piece, x + c * Raw8<X>::kBytes);
+            for (int i = 0; i < V; ++i)
+                if (there(i)) {
+                    copy_shared8<DY>(dy_slot + depth + i * Slots::kDyChunk, 512, dy_at + i * 32 * Raw8<DY>::kBytes);
+                    copy_shared8<X>(x_slot + depth + i * Slots::kXChunk, 512, x_at + i * 32 * Raw8<X>::kBytes);
                     if constexpr (X == kE4m3)
-                        cp_async_4(scale_slot(d, i), p.code_scales + r * p.code_scales_stride + c / 16 * p.scale_col_stride);
+                        copy_shared4(scale_slot + depth + i * 128, scale_at + i * 2 * p.scale_col_stride);
                 }
-            }
+            dy_at += dy_step;
+            x_at += x_step;
+            if constexpr (X == kE4m3)
+                scale_at += share.step * p.code_scales_stride;
         }
+        copied += share.step;
         cp_async_commit();
     };
 
-    float dw[V][8], db[V][8], w[V][8];
+    Pair dw[V][4], db[V][4], w[V][4];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            dw[i][e] = db[i][e] = 0.f;
-            w[i][e] = 1.f;
+        for (int e = 0; e < 4; ++e) {
+            dw[i][e] = db[i][e] = both(0.f);
+            w[i][e] = both(1.f);
         }
-        if (p.weight != nullptr && t + i * stride < chunks)
-            load_param8(p.weight, p.param_type, (t + i * stride) * 8, w[i]);
+        if (p.weight != nullptr && there(i))
+            load_param8<PARAM>(static_cast<const uint8_t *>(p.weight) + (share.chunk + i * 32) * Raw8<PARAM>::kBytes, w[i]);
     }
 #pragma unroll
-    for (int d = 0; d < kDepth - 1; ++d)
-        copy(first + d * step, d);
-    int slot = 0, turn = 0;
-    float rstd = 0.f, mean = 0.f;
-    if (first < p.rows) {
-        rstd = __ldg(p.rstd + first);
+    for (int d = 0; d < Slots::kDepth - 1; ++d)
+        copy(d * Slots::kDepthBytes);
+    uint32_t slot = 0, refill = (Slots::kDepth - 1) * Slots::kDepthBytes, turn = 0;
+    float next_rstd = 0.f, next_mean = 0.f;
+    if (share.row < rows) {
+        next_rstd = __ldg(p.rstd + share.row);
         if (X != kE4m3)
-            mean = __ldg(p.mean + first);
+            next_mean = __ldg(p.mean + share.row);
     }
-    for (int64_t r = first; r < p.rows; r += step, turn ^= 1) {
-        cp_async_wait<kDepth - 2>();
-        const float r_rstd = rstd, r_mean = mean;
-        if (r + step < p.rows) {
-            rstd = __ldg(p.rstd + r + step);
+    uint8_t *dx_at = static_cast<uint8_t *>(p.dx) + int64_t(share.row) * p.width * element_bytes(DY) + share.chunk * Raw8<DY>::kBytes;
+    const int64_t dx_step = int64_t(share.step) * p.width * element_bytes(DY);
+    for (uint32_t r = share.row; r < rows; r += share.step, turn ^= 1) {
+        cp_async_wait<Slots::kDepth - 2>();
+        const float rstd = next_rstd;
+        const Pair minus_mean = both(-next_mean);
+        if (r + share.step < rows) {
+            next_rstd = __ldg(p.rstd + r + share.step);
             if (X != kE4m3)
-                mean = __ldg(p.mean + r + step);
+                next_mean = __ldg(p.mean + r + share.step);
         }
-        // The normalised value is x * up + shift.
-        auto values = [&](int i, float (&g)[8], float (&h)[8]) {
-            slot_row8<DY>(dy_slot(slot, i), piece, g);
-            slot_row8<X>(x_slot(slot, i), piece, h);
-            const float up = X == kE4m3 ? *scale_slot(slot, i) : r_rstd;
+        auto values = [&](int i, Pair (&g)[4], Pair (&h)[4]) {
+            load_shared8<DY>(dy_slot + slot + i * Slots::kDyChunk, 512, g);
+            load_shared8<X>(x_slot + slot + i * Slots::kXChunk, 512, h);
+            const Pair up = both(X == kE4m3 ? load_shared1(scale_slot + slot + i * 128) : rstd);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                h[e] = X == kE4m3 ? h[e] * up : (h[e] - r_mean) * up;
+            for (int e = 0; e < 4; ++e)
+                h[e] = mul2(X == kE4m3 ? h[e] : add2(h[e], minus_mean), up);
         };
-        float a = 0.f, b = 0.f;
+        Pair a = both(0.f), b = both(0.f);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (t + i * stride < chunks) {
-                float g[8], h[8];
-                values(i, g, h);
+        for (int i = 0; i < V; ++i) {
+            Pair g[4], h[4];
+            values(i, g, h);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    dw[i][e] += g[e] * h[e];
-                    db[i][e] += g[e];
-                    const float gw = g[e] * w[i][e];
-                    a += gw;
-                    b += gw * h[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                dw[i][e] = fma2(g[e], h[e], dw[i][e]);
+                db[i][e] = add2(db[i][e], g[e]);
+                g[e] = mul2(g[e], w[i][e]);
+                a = add2(a, g[e]);
+                b = fma2(g[e], h[e], b);
             }
-        const float2 sums = warp_rows ? lanes_sum2(a, b) : block_sum2(a, b, s_sum[turn]);
+        }
+        const float2 sums = warp_rows ? lanes_sum2(total(a), total(b)) : block_sum2(total(a), total(b), s_sum[turn]);
         if (p.dx != nullptr) {
-            const float c1 = sums.x * inv, c2 = sums.y * inv;
-            uint8_t *dx = static_cast<uint8_t *>(p.dx) + r * p.width * int64_t(element_bytes(DY));
+            const Pair c1 = both(-sums.x * inv), c2 = both(-sums.y * inv), up = both(rstd);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (t + i * stride < chunks) {
-                    float g[8], h[8];
+                if (there(i)) {
+                    Pair g[4], h[4];
                     values(i, g, h);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        g[e] = r_rstd * (g[e] * w[i][e] - c1 - h[e] * c2);
-                    store_row8<DY>(dx + (t + i * stride) * Raw8<DY>::kBytes, g);
+                    for (int e = 0; e < 4; ++e)
+                        g[e] = mul2(fma2(h[e], c2, fma2(g[e], w[i][e], c1)), up);
+                    store_row8<DY>(dx_at + i * 32 * Raw8<DY>::kBytes, g);
                 }
+            dx_at += dx_step;
         }
-        // This row's slots were read by this thread alone, so they can be refilled
-        // without a barrier once kDepth - 1 others are ahead of them.
-        const int refill = slot == 0 ? kDepth - 1 : slot - 1;
-        copy(r + (kDepth - 1) * step, refill);
-        slot = slot + 1 == kDepth ? 0 : slot + 1;
+        // The slots to refill held the row before this one, and this thread alone
+        // reads them: no barrier guards the copy.
+        copy(refill);
+        refill = slot;
+        slot = slot + Slots::kDepthBytes == Slots::kDepth * Slots::kDepthBytes ? 0 : slot + Slots::kDepthBytes;
     }
     if (p.dweight == nullptr)
         return;
@@ -460,7 +511,7 @@ __global__ void __launch_bounds__(512) norm_backward_row(const __grid_constant__
     if (!warp_rows) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (const uint32_t c = t + i * stride; c < chunks) {
+            if (const uint32_t c = share.chunk + i * 32; c < chunks) {
                 store_row8<kFp32>(part[0] + c * 8, dw[i]);
                 store_row8<kFp32>(part[1] + c * 8, db[i]);
             }
@@ -474,15 +525,16 @@ __global__ void __launch_bounds__(512) norm_backward_row(const __grid_constant__
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (const uint32_t c = t + i * stride; c < chunks) {
+            if (const uint32_t c = share.chunk + i * 32; c < chunks) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    sums[threadIdx.x / 32 * p.width + c * 8 + e] = which == 0 ? dw[i][e] : db[i][e];
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<float2 *>(sums + threadIdx.x / 32 * p.width + c * 8 + e * 2) =
+                        parts(which == 0 ? dw[i][e] : db[i][e]);
             }
         __syncthreads();
-        for (uint32_t c = threadIdx.x; c < p.width; c += threads) {
+        for (uint32_t c = threadIdx.x; c < p.width; c += blockDim.x) {
             float sum = 0.f;
-            for (uint32_t g = 0; g < threads / 32; ++g)
+            for (uint32_t g = 0; g < blockDim.x / 32; ++g)
                 sum += sums[g * p.width + c];
             part[which][c] = sum;
         }
@@ -495,35 +547,58 @@ uint32_t row_grid(int64_t rows, int num_sms) {
 
 // Whether norm_forward_row's vector accesses are on their boundaries.
 bool whole_chunks(const NormForwardParams &p) {
-    const uint32_t in = p.in_type == kE4m3 ? 8 : 16;
-    if (p.width % 8 != 0 || p.width > 8 * 4 * 1024 || !on_boundary(p.x, in) ||
-        p.x_stride * element_bytes(p.in_type) % in != 0 || !on_boundary(p.weight, 16) || !on_boundary(p.bias, 16))
+    const uint32_t in = 8 * element_bytes(p.in_type), param = 8 * element_bytes(p.param_type);
+    if (p.width % 8 != 0 || p.width > 8 * 4 * 512 || !on_boundary(p.x, in) ||
+        p.x_stride * element_bytes(p.in_type) % in != 0 || !on_boundary(p.weight, param) || !on_boundary(p.bias, param))
         return false;
     return p.in_type != kE4m3 || (p.hidden % 8 == 0 && p.block % 8 == 0);
 }
 
-template <uint32_t IN, uint32_t OUT, int V>
-void forward_row(const NormForwardParams &p, cudaStream_t stream) {
-    const uint32_t chunks = p.width / 8;
-    const bool warp_rows = chunks <= 32 * V;
-    const uint32_t threads = warp_rows ? 128 : ((chunks + V - 1) / V + 31) / 32 * 32;
-    const int64_t grid = warp_rows ? (p.rows + 3) / 4 : p.rows;
-    norm_forward_row<IN, OUT, V><<<uint32_t(grid), threads, 0, stream>>>(p, warp_rows);
+// Blocks of a row kernel that fit an SM at once.
+uint32_t resident(uint32_t threads, uint32_t registers, uint32_t shared) {
+    return std::max(1u, std::min({65536 / (threads * registers), 226 * 1024 / (shared + 1280), 2048 / threads, 16u}));
 }
 
-template <uint32_t IN, uint32_t OUT> void forward(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
-    if (whole_chunks(p)) {
-        const uint32_t chunks = p.width / 8;
-        // By the width alone, so a row's bits do not depend on its batch.
-        if (chunks <= 32)
-            forward_row<IN, OUT, 1>(p, stream);
-        else if (chunks <= 64)
-            forward_row<IN, OUT, 2>(p, stream);
-        else
-            forward_row<IN, OUT, 4>(p, stream);
-        return;
+template <uint32_t IN, uint32_t OUT, uint32_t PARAM, int V, bool FULL, int T>
+cudaError_t forward_row(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    const uint32_t chunks = p.width / 8;
+    const bool warp_rows = chunks <= 32 * V;
+    const uint32_t threads = warp_rows ? 128 : (chunks + 32 * V - 1) / (32 * V) * 32;
+    using Slots = ForwardSlots<IN, V>;
+    const uint32_t shared = threads / 32 * Slots::kDepth * Slots::kDepthBytes;
+    const int64_t groups = warp_rows ? (p.rows + 3) / 4 : p.rows;
+    const uint32_t grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident(threads, T > 384 ? 128 : 80, shared)));
+    const auto kernel = p.keep == kKeepFp8 ? norm_forward_row<IN, OUT, PARAM, V, FULL, true, T>
+                                           : norm_forward_row<IN, OUT, PARAM, V, FULL, false, T>;
+    if (shared > 40 * 1024)
+        if (const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared));
+            rc != cudaSuccess)
+            return rc;
+    kernel<<<grid, threads, shared, stream>>>(p, warp_rows);
+    return cudaSuccess;
+}
+
+template <uint32_t IN, uint32_t OUT, uint32_t PARAM>
+cudaError_t forward_rows(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    // By the width alone, so a row's bits do not depend on its batch.
+    const uint32_t chunks = p.width / 8;
+    return chunks <= 32        ? forward_row<IN, OUT, PARAM, 1, false, 128>(p, num_sms, stream)
+           : chunks <= 64      ? forward_row<IN, OUT, PARAM, 2, false, 128>(p, num_sms, stream)
+           : chunks > 1536     ? forward_row<IN, OUT, PARAM, 4, false, 512>(p, num_sms, stream)
+           : chunks % 128 == 0 ? forward_row<IN, OUT, PARAM, 4, true, 384>(p, num_sms, stream)
+                               : forward_row<IN, OUT, PARAM, 4, false, 384>(p, num_sms, stream);
+}
+
+template <uint32_t IN, uint32_t OUT>
+cudaError_t forward(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    if (!whole_chunks(p)) {
+        norm_forward_any<IN, OUT><<<row_grid(p.rows, num_sms), kRowThreads, 0, stream>>>(p);
+        return cudaGetLastError();
     }
-    norm_forward_any<IN, OUT><<<row_grid(p.rows, num_sms), kRowThreads, 0, stream>>>(p);
+    const cudaError_t rc = OUT != kFp32 && p.weight != nullptr && p.param_type == kFp32
+                               ? forward_rows<IN, OUT, kFp32>(p, num_sms, stream)
+                               : forward_rows<IN, OUT, OUT>(p, num_sms, stream);
+    return rc == cudaSuccess ? cudaGetLastError() : rc;
 }
 
 // How norm_backward_row takes a call; threads == 0: it cannot, and the kernels
@@ -541,12 +616,12 @@ BackwardPlan backward_plan(const NormBackwardParams &p, int num_sms) {
     const void *x = fp8 ? static_cast<const void *>(p.codes) : p.x;
     const int64_t x_stride = fp8 ? p.codes_stride : p.x_stride;
     if (p.width % 8 != 0 || !on_boundary(p.dy, 16) || p.dy_stride * dy_bytes % 16 != 0 || !on_boundary(x, x_boundary) ||
-        x_stride * x_bytes % x_boundary != 0 || !on_boundary(p.weight, 16))
+        x_stride * x_bytes % x_boundary != 0 || !on_boundary(p.weight, p.param_type == kFp32 ? 32 : 16))
         return plan;
     const uint32_t chunks = p.width / 8;
     plan.vectors = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
     plan.warp_rows = chunks <= 32u * plan.vectors;
-    const uint32_t threads = plan.warp_rows ? 256 : ((chunks + plan.vectors - 1) / plan.vectors + 31) / 32 * 32;
+    const uint32_t threads = plan.warp_rows ? 256 : (chunks + 32 * plan.vectors - 1) / (32 * plan.vectors) * 32;
     const uint32_t depth = p.dy_type == kFp32 ? 2 : 3;
     plan.shared = threads * plan.vectors * depth * (8 * (dy_bytes + x_bytes) + (fp8 ? 4 : 0));
     if (plan.warp_rows)
@@ -555,18 +630,28 @@ BackwardPlan backward_plan(const NormBackwardParams &p, int num_sms) {
         return plan;
     plan.threads = threads;
     const int64_t groups = plan.warp_rows ? (p.rows + threads / 32 - 1) / (threads / 32) : p.rows;
-    const uint32_t resident = std::max(1u, std::min({228u * 1024 / (plan.shared + 2048), 65536u / (threads * 128), 8u}));
-    plan.grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident));
+    const uint32_t registers = plan.vectors == 4 && threads <= 384 ? 168 : 128;
+    plan.grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident(threads, registers, plan.shared)));
     return plan;
 }
 
-template <uint32_t X, uint32_t DY, int V>
+template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
 cudaError_t backward_row(const NormBackwardParams &p, const BackwardPlan &plan, cudaStream_t stream) {
-    const cudaError_t rc =
-        cudaFuncSetAttribute(norm_backward_row<X, DY, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (rc == cudaSuccess)
-        norm_backward_row<X, DY, V><<<plan.grid, plan.threads, plan.shared, stream>>>(p, plan.warp_rows);
-    return rc;
+    const auto kernel = norm_backward_row<X, DY, PARAM, V, T>;
+    if (plan.shared > 40 * 1024)
+        if (const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan.shared));
+            rc != cudaSuccess)
+            return rc;
+    kernel<<<plan.grid, plan.threads, plan.shared, stream>>>(p, plan.warp_rows);
+    return cudaSuccess;
+}
+
+template <uint32_t X, uint32_t DY, uint32_t PARAM>
+cudaError_t backward_rows(const NormBackwardParams &p, const BackwardPlan &plan, cudaStream_t stream) {
+    return plan.vectors == 1    ? backward_row<X, DY, PARAM, 1, 256>(p, plan, stream)
+           : plan.vectors == 2  ? backward_row<X, DY, PARAM, 2, 256>(p, plan, stream)
+           : plan.threads > 384 ? backward_row<X, DY, PARAM, 4, 512>(p, plan, stream)
+                                : backward_row<X, DY, PARAM, 4, 384>(p, plan, stream);
 }
 
 template <uint32_t X, uint32_t DY>
@@ -574,9 +659,10 @@ cudaError_t backward(const NormBackwardParams &p, int num_sms, cudaStream_t stre
     const BackwardPlan plan = backward_plan(p, num_sms);
     cudaError_t rc = cudaSuccess;
     if (plan.threads != 0) {
-        rc = plan.vectors == 1   ? backward_row<X, DY, 1>(p, plan, stream)
-             : plan.vectors == 2 ? backward_row<X, DY, 2>(p, plan, stream)
-                                 : backward_row<X, DY, 4>(p, plan, stream);
+        if (DY != kFp32 && p.weight != nullptr && p.param_type == kFp32)
+            rc = backward_rows<X, DY, kFp32>(p, plan, stream);
+        else
+            rc = backward_rows<X, DY, DY>(p, plan, stream);
     } else {
         if (p.dx != nullptr)
             norm_backward_rows_any<X, DY><<<row_grid(p.rows, num_sms), kRowThreads, 0, stream>>>(p);
@@ -592,18 +678,16 @@ cudaError_t backward(const NormBackwardParams &p, int num_sms, cudaStream_t stre
 
 cudaError_t launch_norm_forward(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
     if (p.in_type == kBf16)
-        forward<kBf16, kBf16>(p, num_sms, stream);
-    else if (p.in_type == kFp16)
-        forward<kFp16, kFp16>(p, num_sms, stream);
-    else if (p.in_type == kFp32)
-        forward<kFp32, kFp32>(p, num_sms, stream);
-    else if (p.out_type == kBf16)
-        forward<kE4m3, kBf16>(p, num_sms, stream);
-    else if (p.out_type == kFp16)
-        forward<kE4m3, kFp16>(p, num_sms, stream);
-    else
-        forward<kE4m3, kFp32>(p, num_sms, stream);
-    return cudaGetLastError();
+        return forward<kBf16, kBf16>(p, num_sms, stream);
+    if (p.in_type == kFp16)
+        return forward<kFp16, kFp16>(p, num_sms, stream);
+    if (p.in_type == kFp32)
+        return forward<kFp32, kFp32>(p, num_sms, stream);
+    if (p.out_type == kBf16)
+        return forward<kE4m3, kBf16>(p, num_sms, stream);
+    if (p.out_type == kFp16)
+        return forward<kE4m3, kFp16>(p, num_sms, stream);
+    return forward<kE4m3, kFp32>(p, num_sms, stream);
 }
 
 uint32_t norm_backward_parts(const NormBackwardParams &p, int num_sms) {

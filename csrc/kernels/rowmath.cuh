@@ -100,31 +100,71 @@ template <int LANES = 32> __device__ __forceinline__ float lanes_max(float v) {
     return v;
 }
 
-// Sums of two values over the warp, in every lane.
-__device__ __forceinline__ float2 lanes_sum2(float a, float b) {
+// Sum of one value over the warp, in every lane.
+__device__ __forceinline__ float lanes_sum(float a) {
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) {
+    for (int d = 16; d > 0; d /= 2)
         a += __shfl_xor_sync(0xFFFFFFFFu, a, d);
-        b += __shfl_xor_sync(0xFFFFFFFFu, b, d);
-    }
-    return make_float2(a, b);
+    return a;
 }
 
-// Sums of two values over the block, in every thread.  `shared` holds one
-// float2 per warp and must not be the one of the block's previous call: one
-// barrier then suffices, since every thread has read that one by then.
-__device__ __forceinline__ float2 block_sum2(float a, float b, float2 *shared) {
-    const float2 own = lanes_sum2(a, b);
-    const uint32_t warps = blockDim.x / 32;
-    if (threadIdx.x % 32 == 0)
-        shared[threadIdx.x / 32] = own;
+// Sums of two values over the warp: of a in lanes 0-15, of b in lanes 16-31.
+// The first step swaps halves, so two sums cost five shuffles and not ten.
+__device__ __forceinline__ float lanes_sum_halves(float a, float b) {
+    const bool upper = threadIdx.x & 16;
+    float v = upper ? b : a;
+    v += __shfl_xor_sync(0xFFFFFFFFu, upper ? a : b, 16);
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    return v;
+}
+
+// Sums of two values over the warp, in every lane.
+__device__ __forceinline__ float2 lanes_sum2(float a, float b) {
+    const float v = lanes_sum_halves(a, b), w = __shfl_xor_sync(0xFFFFFFFFu, v, 16);
+    return threadIdx.x & 16 ? make_float2(w, v) : make_float2(v, w);
+}
+
+// Sums over a block of at most 16 warps, in every thread.  `shared` must not be
+// the one of the block's previous call: one barrier then suffices, since every
+// thread has read that one by then.  Entries past the block's warps are zero
+// (clear_sums), so the warps' sums are joined by one load and four shuffles,
+// whatever their number.
+struct WarpSums {
+    float of[2][16];
+};
+
+__device__ __forceinline__ void clear_sums(WarpSums &shared) {
+    for (uint32_t i = threadIdx.x; i < 32; i += blockDim.x)
+        shared.of[i / 16][i % 16] = 0.f;
+}
+
+__device__ __forceinline__ float2 block_sum2(float a, float b, WarpSums &shared) {
+    const uint32_t lane = threadIdx.x % 32;
+    float v = lanes_sum_halves(a, b);
+    if (lane % 16 == 0)
+        shared.of[lane / 16][threadIdx.x / 32] = v;
     __syncthreads();
-    float2 total = make_float2(0.f, 0.f);
-    for (uint32_t w = 0; w < warps; ++w) {
-        total.x += shared[w].x;
-        total.y += shared[w].y;
-    }
-    return total;
+    v = shared.of[lane / 16][lane % 16];
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    const float w = __shfl_xor_sync(0xFFFFFFFFu, v, 16);
+    return lane & 16 ? make_float2(w, v) : make_float2(v, w);
+}
+
+__device__ __forceinline__ float block_sum(float a, WarpSums &shared) {
+    const uint32_t lane = threadIdx.x % 32;
+    a = lanes_sum(a);
+    if (lane == 0)
+        shared.of[0][threadIdx.x / 32] = a;
+    __syncthreads();
+    a = shared.of[0][lane % 16];
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, d);
+    return a;
 }
 
 // Eight adjacent values as they lie in memory: 16 bytes of a 16-bit type, 32
@@ -146,11 +186,52 @@ template <uint32_t TYPE> __device__ __forceinline__ Raw8<TYPE> load_row8(const v
     Raw8<TYPE> r;
     if constexpr (TYPE == kE4m3) {
         asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.v.x), "=r"(r.v.y) : "l"(ptr));
+    } else if constexpr (TYPE == kFp32) {
+        const Vec32 w = ld_nc_na_v8(ptr);
+        r.v = Vec16{w.v[0], w.v[1], w.v[2], w.v[3]};
+        r.v2 = Vec16{w.v[4], w.v[5], w.v[6], w.v[7]};
     } else {
         r.v = ld_nc_na_v4(ptr);
-        if constexpr (TYPE == kFp32)
-            r.v2 = ld_nc_na_v4(static_cast<const uint8_t *>(ptr) + 16);
     }
+    return r;
+}
+
+// Two fp32 values in one register pair, and two operations in one instruction
+// (sm_100).  The kernels over rows are bound by issue slots as much as by
+// memory.  A pair stays one 64-bit value from its unpacking to its rounding:
+// taken apart between operations it costs moves.
+struct Pair {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ Pair pair(float2 f) { return pair(f.x, f.y); }
+__device__ __forceinline__ Pair both(float f) { return pair(f, f); }
+__device__ __forceinline__ float2 parts(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+    return r;
+}
+__device__ __forceinline__ float total(Pair p) {
+    const float2 f = parts(p);
+    return f.x + f.y;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
 
@@ -158,82 +239,112 @@ __device__ __forceinline__ float2 from_bf16x2(uint32_t two) {
     return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xFFFF0000u));
 }
 __device__ __forceinline__ float2 from_fp16x2(uint32_t two) { return __half22float2(*reinterpret_cast<__half2 *>(&two)); }
-
-template <uint32_t TYPE> __device__ __forceinline__ void unpack8(const Raw8<TYPE> &r, float (&x)[8]) {
-    if constexpr (TYPE == kFp32) {
-        const uint32_t w[8] = {r.v.x, r.v.y, r.v.z, r.v.w, r.v2.x, r.v2.y, r.v2.z, r.v2.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            x[e] = __uint_as_float(w[e]);
-    } else if constexpr (TYPE == kE4m3) {
-        const uint32_t w[4] = {r.v.x & 0xFFFFu, r.v.x >> 16, r.v.y & 0xFFFFu, r.v.y >> 16};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = from_e4m3x2(w[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-        }
-    } else {
-        const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = TYPE == kBf16 ? from_bf16x2(w[e]) : from_fp16x2(w[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-        }
-    }
-}
-
 __device__ __forceinline__ uint32_t to_bf16x2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
+__device__ __forceinline__ uint32_t to_fp16x2(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 
-template <uint32_t TYPE> __device__ __forceinline__ void store_row8(void *ptr, const float (&x)[8]) {
+template <uint32_t TYPE> __device__ __forceinline__ void unpack8(const Raw8<TYPE> &r, Pair (&x)[4]) {
     if constexpr (TYPE == kFp32) {
-        st_na_v4(ptr, Vec16{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])});
-        st_na_v4(static_cast<uint8_t *>(ptr) + 16,
-                 Vec16{__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])});
+        x[0] = pair(__uint_as_float(r.v.x), __uint_as_float(r.v.y));
+        x[1] = pair(__uint_as_float(r.v.z), __uint_as_float(r.v.w));
+        x[2] = pair(__uint_as_float(r.v2.x), __uint_as_float(r.v2.y));
+        x[3] = pair(__uint_as_float(r.v2.z), __uint_as_float(r.v2.w));
+    } else if constexpr (TYPE == kE4m3) {
+        x[0] = pair(from_e4m3x2(r.v.x & 0xFFFFu));
+        x[1] = pair(from_e4m3x2(r.v.x >> 16));
+        x[2] = pair(from_e4m3x2(r.v.y & 0xFFFFu));
+        x[3] = pair(from_e4m3x2(r.v.y >> 16));
+    } else {
+        const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = pair(TYPE == kBf16 ? from_bf16x2(w[e]) : from_fp16x2(w[e]));
+    }
+}
+
+template <uint32_t TYPE> __device__ __forceinline__ void store_row8(void *ptr, const Pair (&x)[4]) {
+    if constexpr (TYPE == kFp32) {
+        Vec32 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w.v[2 * e] = __float_as_uint(parts(x[e]).x);
+            w.v[2 * e + 1] = __float_as_uint(parts(x[e]).y);
+        }
+        st_v8(ptr, w);
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (TYPE == kBf16) {
-                w[e] = to_bf16x2(x[2 * e], x[2 * e + 1]);
-            } else {
-                const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-                w[e] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-        }
+        for (int e = 0; e < 4; ++e)
+            w[e] = TYPE == kBf16 ? to_bf16x2(parts(x[e]).x, parts(x[e]).y) : to_fp16x2(parts(x[e]).x, parts(x[e]).y);
         st_na_v4(ptr, Vec16{w[0], w[1], w[2], w[3]});
     }
 }
 
-// Eight codes of values already divided by their scale.
-__device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float down) {
+// Eight codes of values that are finite or NaN, divided by their scale.
+__device__ __forceinline__ uint2 to_e4m3x8(const Pair (&x)[4], float down) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        w[e] = to_e4m3x2(x[2 * e] * down, x[2 * e + 1] * down);
+        w[e] = __nv_cvt_float2_to_fp8x2(parts(mul2(x[e], both(down))), __NV_SATFINITE, __NV_E4M3);
     return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
-// Eight adjacent parameters (16-byte aligned); their type is uniform over the launch.
-__device__ __forceinline__ void load_param8(const void *ptr, uint32_t type, uint32_t at, float (&x)[8]) {
-    if (type == kFp32) {
-        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(ptr) + at);
-        const float4 a = __ldg(q), b = __ldg(q + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// Eight adjacent parameters (on a 16-byte boundary, fp32 on a 32-byte one), kept in L1.
+template <uint32_t TYPE> __device__ __forceinline__ void load_param8(const uint8_t *ptr, Pair (&x)[4]) {
+    Raw8<TYPE> r;
+    if constexpr (TYPE == kFp32) {
+        asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r.v.x), "=r"(r.v.y), "=r"(r.v.z), "=r"(r.v.w), "=r"(r.v2.x), "=r"(r.v2.y), "=r"(r.v2.z),
+                       "=r"(r.v2.w)
+                     : "l"(ptr));
     } else {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(ptr) + at));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = type == kBf16 ? from_bf16x2(w[e]) : from_fp16x2(w[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-        }
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(ptr));
+        r.v = Vec16{a.x, a.y, a.z, a.w};
     }
+    unpack8<TYPE>(r, x);
+}
+
+// Eight values from shared memory; fp32's second half lies `half` bytes on.
+template <uint32_t TYPE> __device__ __forceinline__ void load_shared8(uint32_t at, uint32_t half, Pair (&x)[4]) {
+    Raw8<TYPE> r;
+    if constexpr (TYPE == kE4m3) {
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.v.x), "=r"(r.v.y) : "r"(at));
+    } else {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.v.x), "=r"(r.v.y), "=r"(r.v.z), "=r"(r.v.w)
+                     : "r"(at));
+        if constexpr (TYPE == kFp32)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r.v2.x), "=r"(r.v2.y), "=r"(r.v2.z), "=r"(r.v2.w)
+                         : "r"(at + half));
+    }
+    unpack8<TYPE>(r, x);
+}
+
+// The asynchronous copy that load_shared8 reads (completes with cp.async.wait_group).
+template <uint32_t TYPE> __device__ __forceinline__ void copy_shared8(uint32_t at, uint32_t half, const uint8_t *src) {
+    if constexpr (TYPE == kE4m3) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(src) : "memory");
+    } else {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
+        if constexpr (TYPE == kFp32)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + half), "l"(src + 16) : "memory");
+    }
+}
+
+__device__ __forceinline__ float load_shared1(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+
+__device__ __forceinline__ void copy_shared4(uint32_t at, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(src) : "memory");
 }
 
 inline bool on_boundary(const void *ptr, uint32_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes == 0; }
