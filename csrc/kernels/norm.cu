@@ -10,6 +10,7 @@
 
 #include "readout.h"
 #include "rowmath.cuh"
+#include "tensor.cuh"
 
 namespace engram {
 
@@ -111,27 +112,24 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
 // chunks of its row, lane l those with l = c % 32, so all of a thread's offsets
 // are constants; FULL: every thread has V of them.  A row takes a block of
 // warps or, with at most 32 V chunks, one warp of a block.  Blocks stay and
-// take every gridDim-th row (warp row).  What a thread needs of the rows to
-// come it copies itself into its own slots of shared memory, slot_depth - 1
-// rows ahead, so no barrier guards the copies and they cost no registers.
-constexpr int slot_depth(uint32_t type) { return type == kFp32 ? 2 : 3; }
+// take every gridDim-th row (warp row).  One thread copies the rows to come
+// into a ring in shared memory by bulk copies (per-thread copies of 4 and 8
+// bytes kept the load/store unit busy two thirds of the time).
+constexpr int ring_depth(uint32_t type) { return type == kFp32 ? 2 : 3; }
+constexpr uint64_t kWaitNs = 2000000000ull;  // far above any legal wait
+constexpr int kMaxWarps = 16;
 
 struct RowShare {
-    uint32_t row, step, chunk;  // first row, rows to the next, first chunk
+    uint32_t row, step, chunk, group;  // first row, rows to the next, first chunk, ring
+    bool leader;                       // issues its ring's copies
     __device__ __forceinline__ RowShare(bool warp_rows, int vectors) {
         const uint32_t warp = threadIdx.x / 32, warps = blockDim.x / 32;
         row = warp_rows ? blockIdx.x * warps + warp : blockIdx.x;
         step = warp_rows ? gridDim.x * warps : gridDim.x;
         chunk = threadIdx.x % 32 + (warp_rows ? 0 : warp * 32 * vectors);
+        group = warp_rows ? warp : 0;
+        leader = warp_rows ? threadIdx.x % 32 == 0 : threadIdx.x == 0;
     }
-};
-
-// A warp's bytes of one depth of slots: V x 32 chunks, then their scales.
-template <uint32_t IN, int V> struct ForwardSlots {
-    static constexpr int kDepth = slot_depth(IN);
-    static constexpr uint32_t kChunk = 32 * Raw8<IN>::kBytes;
-    static constexpr uint32_t kScales = V * kChunk;
-    static constexpr uint32_t kDepthBytes = kScales + (IN == kE4m3 ? V * 128 : 0);
 };
 
 // The row is read once and held in registers between the two sums and the
@@ -140,52 +138,59 @@ template <uint32_t IN, int V> struct ForwardSlots {
 template <uint32_t IN, uint32_t OUT, uint32_t PARAM, int V, bool FULL, bool FP8, int T>
 __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     norm_forward_row(const __grid_constant__ NormForwardParams p, bool warp_rows) {
-    using Slots = ForwardSlots<IN, V>;
-    extern __shared__ __align__(16) uint8_t s_slots[];
+    constexpr int kDepth = ring_depth(IN);
+    extern __shared__ __align__(16) uint8_t s_ring[];
     __shared__ WarpSums s_sum[2];
+    __shared__ uint64_t s_full[kMaxWarps][kDepth];
+    const RowShare share(warp_rows, V);
     clear_sums(s_sum[0]);
     clear_sums(s_sum[1]);
+    if (share.leader) {
+        for (int d = 0; d < kDepth; ++d)
+            mbar_init(&s_full[share.group][d], 1);
+        fence_mbar_init();
+    }
     __syncthreads();
-    const RowShare share(warp_rows, V);
     const uint32_t chunks = p.width / 8, rows = uint32_t(p.rows), lane = threadIdx.x % 32;
     const float inv = 1.f / float(p.width);
-    const uint32_t warp_slots = smem_addr(s_slots) + threadIdx.x / 32 * (Slots::kDepthBytes * Slots::kDepth);
-    const uint32_t x_slot = warp_slots + lane * (IN == kE4m3 ? 8 : 16), scale_slot = warp_slots + Slots::kScales + lane * 4;
+    const uint32_t row_bytes = chunks * Raw8<IN>::kBytes;
+    uint8_t *ring = s_ring + share.group * kDepth * row_bytes;
+    const uint32_t x_slot = smem_addr(ring) + share.chunk * Raw8<IN>::kBytes;
     const auto there = [&](int i) { return FULL || share.chunk + i * 32 < chunks; };
 
-    const uint8_t *x_at = static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(IN)) +
-                          share.chunk * Raw8<IN>::kBytes;
     const int64_t x_step = share.step * p.x_stride * int64_t(element_bytes(IN));
+    const uint8_t *x_at = static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(IN));
+    uint32_t copied = share.row;
+    auto copy = [&](uint32_t slot) {  // the leader's
+        if (copied < rows) {
+            mbar_arrive_expect_tx(&s_full[share.group][slot], row_bytes);
+            bulk_load(ring + slot * row_bytes, x_at, row_bytes, &s_full[share.group][slot]);
+        }
+        copied += share.step;
+        x_at += x_step;
+    };
+    if (share.leader)
+        for (int d = 0; d < kDepth; ++d)
+            copy(d);
     const float *scale_at = IN == kE4m3 ? p.scales + share.row * p.scale_row_stride : nullptr;
     uint32_t pack[V];
+    float next_scale[V];
+    auto load_scales = [&] {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            next_scale[i] = there(i) ? __ldg(scale_at + pack[i] * p.scale_col_stride) : 0.f;
+        scale_at += share.step * p.scale_row_stride;
+    };
     if constexpr (IN == kE4m3) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const uint32_t column = (share.chunk + i * 32) * 8, entry = column / p.hidden;
             pack[i] = entry * p.packs + (column - entry * p.hidden) / p.block;
         }
+        if (share.row < rows)
+            load_scales();
     }
-    uint32_t copied = share.row;
-    auto copy = [&](uint32_t depth) {
-        if (copied < rows) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (there(i)) {
-                    copy_shared8<IN>(x_slot + depth + i * Slots::kChunk, 512, x_at + i * 32 * Raw8<IN>::kBytes);
-                    if constexpr (IN == kE4m3)
-                        copy_shared4(scale_slot + depth + i * 128, scale_at + pack[i] * p.scale_col_stride);
-                }
-            x_at += x_step;
-            if constexpr (IN == kE4m3)
-                scale_at += share.step * p.scale_row_stride;
-        }
-        copied += share.step;
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int d = 0; d < Slots::kDepth - 1; ++d)
-        copy(d * Slots::kDepthBytes);
-    uint32_t slot = 0, refill = (Slots::kDepth - 1) * Slots::kDepthBytes;
+    uint32_t slot = 0, phase = 0;
     uint8_t *y_at = static_cast<uint8_t *>(p.y) + int64_t(share.row) * p.width * element_bytes(OUT) + share.chunk * Raw8<OUT>::kBytes;
     const int64_t y_step = int64_t(share.step) * p.width * element_bytes(OUT);
     const uint8_t *w_at = static_cast<const uint8_t *>(p.weight) + share.chunk * Raw8<PARAM>::kBytes;
@@ -193,27 +198,34 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     const uint32_t blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
     const bool affine = p.weight != nullptr, shifted = p.bias != nullptr;
     for (uint32_t r = share.row; r < rows; r += share.step) {
-        cp_async_wait<Slots::kDepth - 2>();
+        if (!mbar_wait(&s_full[share.group][slot], phase, kWaitNs)) {
+            st_release_sys_u32(p.fault, kPipelineTimeout);
+            return;
+        }
         Pair x[V][4];
         Pair a = both(0.f), b = both(0.f);
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (there(i)) {
-                load_shared8<IN>(x_slot + slot + i * Slots::kChunk, 512, x[i]);
+                load_shared8<IN>(x_slot + slot * row_bytes + i * 32 * Raw8<IN>::kBytes, x[i]);
                 if constexpr (IN == kE4m3) {
-                    const Pair scale = both(load_shared1(scale_slot + slot + i * 128));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        x[i][e] = mul2(x[i][e], scale);
+                        x[i][e] = mul2(x[i][e], both(next_scale[i]));
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     a = add2(a, x[i][e]);
             }
-        copy(refill);  // the row before this one was there, and this thread alone read it
-        refill = slot;
-        slot = slot + Slots::kDepthBytes == Slots::kDepth * Slots::kDepthBytes ? 0 : slot + Slots::kDepthBytes;
+        if constexpr (IN == kE4m3)
+            if (r + share.step < rows)
+                load_scales();
+        // Every thread of the row has read its slot when the first sum is there.
         const float mean = (warp_rows ? lanes_sum(total(a)) : block_sum(total(a), s_sum[0])) * inv;
+        if (share.leader)
+            copy(slot);
+        slot = slot + 1 == kDepth ? 0 : slot + 1;
+        phase ^= slot == 0 ? 1 : 0;
         const Pair minus_mean = both(-mean);
         a = both(0.f);
 #pragma unroll
@@ -229,7 +241,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
         const float2 sums = warp_rows ? lanes_sum2(total(a), total(b)) : block_sum2(total(a), total(b), s_sum[1]);
         const float shift = sums.x * inv;
         const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
-        if (share.chunk == 0 && p.keep != kKeepNothing) {
+        if (share.leader && p.keep != kKeepNothing) {
             if (p.keep == kKeepStats)
                 p.mean[r] = mean + shift;
             p.rstd[r] = rstd;
@@ -373,62 +385,57 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
 // Rows of whole chunks (as in norm_forward_row), dx and the column sums in one
 // pass over memory.  A thread owns the same columns in all rows of its block:
 // its sums for dweight and dbias stay in registers, and each block leaves one
-// part of them.  Its slots: dy's chunks, the kept rows' chunks, their scales.
-template <uint32_t X, uint32_t DY, int V> struct BackwardSlots {
-    static constexpr int kDepth = slot_depth(DY);
-    static constexpr uint32_t kDyChunk = 32 * Raw8<DY>::kBytes, kXChunk = 32 * Raw8<X>::kBytes;
-    static constexpr uint32_t kX = V * kDyChunk, kScales = kX + V * kXChunk;
-    static constexpr uint32_t kDepthBytes = kScales + (X == kE4m3 ? V * 128 : 0);
-};
-
+// part of them.  A ring slot holds dy's row, then the kept one, each with room
+// for a chunk in every place; what no chunk fills is zero and adds nothing.
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
 __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
-    using Slots = BackwardSlots<X, DY, V>;
-    extern __shared__ __align__(16) uint8_t s_slots[];
+    constexpr int kDepth = ring_depth(DY);
+    extern __shared__ __align__(16) uint8_t s_ring[];
     __shared__ WarpSums s_sum[2];
+    __shared__ uint64_t s_full[kMaxWarps][kDepth];
+    const RowShare share(warp_rows, V);
     clear_sums(s_sum[0]);
     clear_sums(s_sum[1]);
-    const RowShare share(warp_rows, V);
-    const uint32_t chunks = p.width / 8, rows = uint32_t(p.rows), lane = threadIdx.x % 32;
+    if (share.leader) {
+        for (int d = 0; d < kDepth; ++d)
+            mbar_init(&s_full[share.group][d], 1);
+        fence_mbar_init();
+    }
+    const uint32_t chunks = p.width / 8, rows = uint32_t(p.rows);
     const float inv = 1.f / float(p.width);
-    const uint32_t warp_bytes = Slots::kDepthBytes * Slots::kDepth;
-    const uint32_t warp_slots = smem_addr(s_slots) + threadIdx.x / 32 * warp_bytes;
-    const uint32_t dy_slot = warp_slots + lane * 16, x_slot = warp_slots + Slots::kX + lane * (X == kE4m3 ? 8 : 16);
-    const uint32_t scale_slot = warp_slots + Slots::kScales + lane * 4;
-    const auto there = [&](int i) { return share.chunk + i * 32 < chunks; };
-    // What no chunk fills is zero, so that it adds nothing.
-    for (uint32_t at = threadIdx.x * 4; at < warp_bytes * (blockDim.x / 32); at += blockDim.x * 4)
-        *reinterpret_cast<uint32_t *>(s_slots + at) = 0;
+    const uint32_t places = (warp_rows ? 32 : blockDim.x) * V;
+    const uint32_t x_offset = places * Raw8<DY>::kBytes, slot_bytes = places * (Raw8<DY>::kBytes + Raw8<X>::kBytes);
+    const uint32_t groups = warp_rows ? blockDim.x / 32 : 1;
+    for (uint32_t at = threadIdx.x * 16; at < groups * kDepth * slot_bytes; at += blockDim.x * 16)
+        *reinterpret_cast<uint4 *>(s_ring + at) = make_uint4(0, 0, 0, 0);
+    fence_async_shared();
     __syncthreads();
+    uint8_t *ring = s_ring + share.group * kDepth * slot_bytes;
+    const uint32_t dy_slot = smem_addr(ring) + share.chunk * Raw8<DY>::kBytes;
+    const uint32_t x_slot = smem_addr(ring) + x_offset + share.chunk * Raw8<X>::kBytes;
+    const auto there = [&](int i) { return share.chunk + i * 32 < chunks; };
 
-    const uint8_t *dy_at = static_cast<const uint8_t *>(p.dy) + share.row * p.dy_stride * int64_t(element_bytes(DY)) +
-                           share.chunk * Raw8<DY>::kBytes;
+    const uint8_t *dy_at = static_cast<const uint8_t *>(p.dy) + share.row * p.dy_stride * int64_t(element_bytes(DY));
     const uint8_t *x_at = X == kE4m3 ? p.codes + share.row * p.codes_stride
                                      : static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(X));
-    x_at += share.chunk * Raw8<X>::kBytes;
-    const float *scale_at =
-        X == kE4m3 ? p.code_scales + share.row * p.code_scales_stride + share.chunk / 16 * p.scale_col_stride : nullptr;
     const int64_t dy_step = share.step * p.dy_stride * int64_t(element_bytes(DY));
     const int64_t x_step = X == kE4m3 ? share.step * p.codes_stride : share.step * p.x_stride * int64_t(element_bytes(X));
+    const uint32_t dy_bytes = chunks * Raw8<DY>::kBytes, x_bytes = (chunks * Raw8<X>::kBytes + 15) / 16 * 16;
     uint32_t copied = share.row;
-    auto copy = [&](uint32_t depth) {
+    auto copy = [&](uint32_t slot) {  // the leader's
         if (copied < rows) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (there(i)) {
-                    copy_shared8<DY>(dy_slot + depth + i * Slots::kDyChunk, 512, dy_at + i * 32 * Raw8<DY>::kBytes);
-                    copy_shared8<X>(x_slot + depth + i * Slots::kXChunk, 512, x_at + i * 32 * Raw8<X>::kBytes);
-                    if constexpr (X == kE4m3)
-                        copy_shared4(scale_slot + depth + i * 128, scale_at + i * 2 * p.scale_col_stride);
-                }
-            dy_at += dy_step;
-            x_at += x_step;
-            if constexpr (X == kE4m3)
-                scale_at += share.step * p.code_scales_stride;
+            uint64_t *full = &s_full[share.group][slot];
+            mbar_arrive_expect_tx(full, dy_bytes + x_bytes);
+            bulk_load(ring + slot * slot_bytes, dy_at, dy_bytes, full);
+            bulk_load(ring + slot * slot_bytes + x_offset, x_at, x_bytes, full);
         }
         copied += share.step;
-        cp_async_commit();
+        dy_at += dy_step;
+        x_at += x_step;
     };
+    if (share.leader)
+        for (int d = 0; d < kDepth - 1; ++d)
+            copy(d);
 
     Pair dw[V][4], db[V][4], w[V][4];
 #pragma unroll
@@ -441,31 +448,44 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
         if (p.weight != nullptr && there(i))
             load_param8<PARAM>(static_cast<const uint8_t *>(p.weight) + (share.chunk + i * 32) * Raw8<PARAM>::kBytes, w[i]);
     }
+    const float *scale_at =
+        X == kE4m3 ? p.code_scales + share.row * p.code_scales_stride + share.chunk / 16 * p.scale_col_stride : nullptr;
+    float next_rstd = 0.f, next_mean = 0.f, next_scale[V];
+    auto load_stats = [&](uint32_t r) {
+        next_rstd = __ldg(p.rstd + r);
+        if constexpr (X == kE4m3) {
 #pragma unroll
-    for (int d = 0; d < Slots::kDepth - 1; ++d)
-        copy(d * Slots::kDepthBytes);
-    uint32_t slot = 0, refill = (Slots::kDepth - 1) * Slots::kDepthBytes, turn = 0;
-    float next_rstd = 0.f, next_mean = 0.f;
-    if (share.row < rows) {
-        next_rstd = __ldg(p.rstd + share.row);
-        if (X != kE4m3)
-            next_mean = __ldg(p.mean + share.row);
-    }
+            for (int i = 0; i < V; ++i)
+                next_scale[i] = there(i) ? __ldg(scale_at + i * 2 * p.scale_col_stride) : 0.f;
+            scale_at += share.step * p.code_scales_stride;
+        } else {
+            next_mean = __ldg(p.mean + r);
+        }
+    };
+    if (share.row < rows)
+        load_stats(share.row);
+    uint32_t slot = 0, phase = 0, turn = 0, refill = kDepth - 1;
     uint8_t *dx_at = static_cast<uint8_t *>(p.dx) + int64_t(share.row) * p.width * element_bytes(DY) + share.chunk * Raw8<DY>::kBytes;
     const int64_t dx_step = int64_t(share.step) * p.width * element_bytes(DY);
     for (uint32_t r = share.row; r < rows; r += share.step, turn ^= 1) {
-        cp_async_wait<Slots::kDepth - 2>();
         const float rstd = next_rstd;
         const Pair minus_mean = both(-next_mean);
-        if (r + share.step < rows) {
-            next_rstd = __ldg(p.rstd + r + share.step);
-            if (X != kE4m3)
-                next_mean = __ldg(p.mean + r + share.step);
+        float scale[V];
+        if constexpr (X == kE4m3) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                scale[i] = next_scale[i];
+        }
+        if (r + share.step < rows)
+            load_stats(r + share.step);
+        if (!mbar_wait(&s_full[share.group][slot], phase, kWaitNs)) {
+            st_release_sys_u32(p.fault, kPipelineTimeout);
+            return;
         }
         auto values = [&](int i, Pair (&g)[4], Pair (&h)[4]) {
-            load_shared8<DY>(dy_slot + slot + i * Slots::kDyChunk, 512, g);
-            load_shared8<X>(x_slot + slot + i * Slots::kXChunk, 512, h);
-            const Pair up = both(X == kE4m3 ? load_shared1(scale_slot + slot + i * 128) : rstd);
+            load_shared8<DY>(dy_slot + slot * slot_bytes + i * 32 * Raw8<DY>::kBytes, g);
+            load_shared8<X>(x_slot + slot * slot_bytes + i * 32 * Raw8<X>::kBytes, h);
+            const Pair up = both(X == kE4m3 ? scale[i] : rstd);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 h[e] = mul2(X == kE4m3 ? h[e] : add2(h[e], minus_mean), up);
@@ -485,6 +505,9 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
             }
         }
         const float2 sums = warp_rows ? lanes_sum2(total(a), total(b)) : block_sum2(total(a), total(b), s_sum[turn]);
+        // Past the sum every thread is done with the row before this one.
+        if (share.leader)
+            copy(refill);
         if (p.dx != nullptr) {
             const Pair c1 = both(-sums.x * inv), c2 = both(-sums.y * inv), up = both(rstd);
 #pragma unroll
@@ -499,11 +522,9 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
                 }
             dx_at += dx_step;
         }
-        // The slots to refill held the row before this one, and this thread alone
-        // reads them: no barrier guards the copy.
-        copy(refill);
         refill = slot;
-        slot = slot + Slots::kDepthBytes == Slots::kDepth * Slots::kDepthBytes ? 0 : slot + Slots::kDepthBytes;
+        slot = slot + 1 == kDepth ? 0 : slot + 1;
+        phase ^= slot == 0 ? 1 : 0;
     }
     if (p.dweight == nullptr)
         return;
@@ -518,8 +539,7 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
         return;
     }
     // Warp rows: the block's warps hold sums of the same columns.
-    cp_async_wait<0>();
-    float *sums = reinterpret_cast<float *>(s_slots);
+    float *sums = reinterpret_cast<float *>(s_ring);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -545,11 +565,11 @@ uint32_t row_grid(int64_t rows, int num_sms) {
     return uint32_t(rows < int64_t(num_sms) * 8 ? rows : int64_t(num_sms) * 8);
 }
 
-// Whether norm_forward_row's vector accesses are on their boundaries.
+// Whether norm_forward_row's copies and vectors are on their boundaries.
 bool whole_chunks(const NormForwardParams &p) {
-    const uint32_t in = 8 * element_bytes(p.in_type), param = 8 * element_bytes(p.param_type);
-    if (p.width % 8 != 0 || p.width > 8 * 4 * 512 || !on_boundary(p.x, in) ||
-        p.x_stride * element_bytes(p.in_type) % in != 0 || !on_boundary(p.weight, param) || !on_boundary(p.bias, param))
+    const uint32_t size = element_bytes(p.in_type), param = 8 * element_bytes(p.param_type);
+    if (p.width % 8 != 0 || p.width > 8 * 4 * 512 || p.width * size % 16 != 0 || !on_boundary(p.x, 16) ||
+        p.x_stride * size % 16 != 0 || !on_boundary(p.weight, param) || !on_boundary(p.bias, param))
         return false;
     return p.in_type != kE4m3 || (p.hidden % 8 == 0 && p.block % 8 == 0);
 }
@@ -564,8 +584,7 @@ cudaError_t forward_row(const NormForwardParams &p, int num_sms, cudaStream_t st
     const uint32_t chunks = p.width / 8;
     const bool warp_rows = chunks <= 32 * V;
     const uint32_t threads = warp_rows ? 128 : (chunks + 32 * V - 1) / (32 * V) * 32;
-    using Slots = ForwardSlots<IN, V>;
-    const uint32_t shared = threads / 32 * Slots::kDepth * Slots::kDepthBytes;
+    const uint32_t shared = (warp_rows ? 4 : 1) * ring_depth(IN) * p.width * element_bytes(IN);
     const int64_t groups = warp_rows ? (p.rows + 3) / 4 : p.rows;
     const uint32_t grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident(threads, T > 384 ? 128 : 80, shared)));
     const auto kernel = p.keep == kKeepFp8 ? norm_forward_row<IN, OUT, PARAM, V, FULL, true, T>
@@ -612,18 +631,17 @@ struct BackwardPlan {
 BackwardPlan backward_plan(const NormBackwardParams &p, int num_sms) {
     BackwardPlan plan{};
     const bool fp8 = p.keep == kKeepFp8;
-    const uint32_t dy_bytes = element_bytes(p.dy_type), x_bytes = fp8 ? 1 : dy_bytes, x_boundary = fp8 ? 8 : 16;
+    const uint32_t dy_bytes = element_bytes(p.dy_type), x_bytes = fp8 ? 1 : dy_bytes;
     const void *x = fp8 ? static_cast<const void *>(p.codes) : p.x;
     const int64_t x_stride = fp8 ? p.codes_stride : p.x_stride;
-    if (p.width % 8 != 0 || !on_boundary(p.dy, 16) || p.dy_stride * dy_bytes % 16 != 0 || !on_boundary(x, x_boundary) ||
-        x_stride * x_bytes % x_boundary != 0 || !on_boundary(p.weight, p.param_type == kFp32 ? 32 : 16))
+    if (p.width % 8 != 0 || !on_boundary(p.dy, 16) || p.dy_stride * dy_bytes % 16 != 0 || !on_boundary(x, 16) ||
+        x_stride * x_bytes % 16 != 0 || p.width * x_bytes % 16 != 0 || !on_boundary(p.weight, p.param_type == kFp32 ? 32 : 16))
         return plan;
     const uint32_t chunks = p.width / 8;
     plan.vectors = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
     plan.warp_rows = chunks <= 32u * plan.vectors;
     const uint32_t threads = plan.warp_rows ? 256 : (chunks + 32 * plan.vectors - 1) / (32 * plan.vectors) * 32;
-    const uint32_t depth = p.dy_type == kFp32 ? 2 : 3;
-    plan.shared = threads * plan.vectors * depth * (8 * (dy_bytes + x_bytes) + (fp8 ? 4 : 0));
+    plan.shared = threads * plan.vectors * ring_depth(p.dy_type) * 8 * (dy_bytes + x_bytes);
     if (plan.warp_rows)
         plan.shared = std::max(plan.shared, threads / 32 * p.width * 4);
     if (threads > 512 || plan.shared > 200 * 1024)

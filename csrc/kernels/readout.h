@@ -33,6 +33,7 @@ struct NormForwardParams {
     float *mean, *rstd;      // [rows]; mean with kKeepStats, rstd with either
     uint8_t *codes;          // kKeepFp8: [rows][codes_stride]
     float *code_scales;      // kKeepFp8: [rows][ceil(width / 128)]
+    uint32_t *fault;         // host-mapped: set when a wait ran out
     int64_t rows, x_stride, codes_stride, scale_row_stride, scale_col_stride;
     uint32_t width, hidden, packs, block;
     uint32_t in_type, out_type, param_type, keep;
@@ -52,6 +53,7 @@ struct NormBackwardParams {
     void *dx;                // nullptr: not wanted
     void *dweight, *dbias;   // nullptr: not wanted (both or neither)
     float *partial;          // [2][parts][width] of dweight and dbias sums
+    uint32_t *fault;         // host-mapped: set when a wait ran out
     int64_t rows, dy_stride, x_stride, codes_stride, code_scales_stride, scale_col_stride;
     uint32_t width, parts;
     uint32_t dy_type, x_type, param_type, keep;

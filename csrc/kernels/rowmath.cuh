@@ -309,8 +309,8 @@ template <uint32_t TYPE> __device__ __forceinline__ void load_param8(const uint8
     unpack8<TYPE>(r, x);
 }
 
-// Eight values from shared memory; fp32's second half lies `half` bytes on.
-template <uint32_t TYPE> __device__ __forceinline__ void load_shared8(uint32_t at, uint32_t half, Pair (&x)[4]) {
+// Eight values from shared memory.
+template <uint32_t TYPE> __device__ __forceinline__ void load_shared8(uint32_t at, Pair (&x)[4]) {
     Raw8<TYPE> r;
     if constexpr (TYPE == kE4m3) {
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.v.x), "=r"(r.v.y) : "r"(at));
@@ -321,30 +321,9 @@ template <uint32_t TYPE> __device__ __forceinline__ void load_shared8(uint32_t a
         if constexpr (TYPE == kFp32)
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(r.v2.x), "=r"(r.v2.y), "=r"(r.v2.z), "=r"(r.v2.w)
-                         : "r"(at + half));
+                         : "r"(at + 16));
     }
     unpack8<TYPE>(r, x);
-}
-
-// The asynchronous copy that load_shared8 reads (completes with cp.async.wait_group).
-template <uint32_t TYPE> __device__ __forceinline__ void copy_shared8(uint32_t at, uint32_t half, const uint8_t *src) {
-    if constexpr (TYPE == kE4m3) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(src) : "memory");
-    } else {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
-        if constexpr (TYPE == kFp32)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + half), "l"(src + 16) : "memory");
-    }
-}
-
-__device__ __forceinline__ float load_shared1(uint32_t at) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-    return v;
-}
-
-__device__ __forceinline__ void copy_shared4(uint32_t at, const float *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(src) : "memory");
 }
 
 inline bool on_boundary(const void *ptr, uint32_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes == 0; }

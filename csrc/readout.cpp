@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <array>
+#include <atomic>
 #include <cstring>
 #include <mutex>
 #include <optional>
@@ -98,30 +99,32 @@ bool on_16_bytes(const Tensor &t, int64_t size) {
 }
 
 // One host-mapped word per device that a kernel sets when one of its bounded
-// waits ran out (its results are then not to be used); it is read before every
-// launch without synchronising.
-uint32_t *fault_word(int device) {
+// waits ran out (its results are then not to be used).  It is read before every
+// launch, without synchronising, and a set one refuses all further ones.
+uint32_t *healthy_word(int device) {
+    static std::array<std::atomic<uint32_t *>, 64> words{};
     static std::mutex mutex;
-    static std::array<uint32_t *, 64> words{};
     check(device >= 0 && device < int(words.size()), "device index out of range");
-    std::lock_guard<std::mutex> lock(mutex);
-    if (words[device] == nullptr) {
-        // Allowed while a graph is captured: the allocation is no part of it.
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
-        void *word = nullptr;
-        const cudaError_t rc = cudaHostAlloc(&word, 64, cudaHostAllocMapped | cudaHostAllocPortable);
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        check_cuda(rc, "allocate fault word");
-        std::memset(word, 0, 64);
-        words[device] = static_cast<uint32_t *>(word);
+    uint32_t *word = words[device].load(std::memory_order_acquire);
+    if (word == nullptr) {
+        std::lock_guard<std::mutex> lock(mutex);
+        word = words[device].load(std::memory_order_relaxed);
+        if (word == nullptr) {
+            // Allowed while a graph is captured: the allocation is no part of it.
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+            void *fresh = nullptr;
+            const cudaError_t rc = cudaHostAlloc(&fresh, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            check_cuda(rc, "allocate fault word");
+            std::memset(fresh, 0, 64);
+            word = static_cast<uint32_t *>(fresh);
+            words[device].store(word, std::memory_order_release);
+        }
     }
-    return words[device];
-}
-
-void need_healthy(const uint32_t *fault) {
-    check(*static_cast<const volatile uint32_t *>(fault) == 0,
-          "an earlier weight gradient on this GPU gave up waiting for its pipeline; its results are invalid");
+    check(*static_cast<const volatile uint32_t *>(word) == 0,
+          "an earlier read-out kernel on this GPU gave up waiting for its own copies; its results are invalid");
+    return word;
 }
 
 // (y, codes | None, scales | None, mean | None, rstd | None)
@@ -187,6 +190,7 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
         p.param_type = weight ? element_type(weight->scalar_type()) : 0;
         p.keep = keep;
         p.eps = float(eps);
+        p.fault = healthy_word(device);
         check_cuda(launch_norm_forward(p, sm_count(device), at::cuda::getCurrentCUDAStream(device).stream()),
                    "launch layer norm");
     }
@@ -256,6 +260,7 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
     p.x_type = element_type(kept.scalar_type());
     p.param_type = weight ? element_type(weight->scalar_type()) : 0;
     p.keep = fp8 ? kKeepFp8 : kKeepStats;
+    p.fault = healthy_word(device);
     const int sms = sm_count(device);
     if (params) {
         p.parts = norm_backward_parts(p, sms);
@@ -340,8 +345,7 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
             dbias->zero_();
         return py::make_tuple(dweight, dbias);
     }
-    uint32_t *fault = fault_word(device);
-    need_healthy(fault);
+    uint32_t *fault = healthy_word(device);
     // Tiled copies want rows on 16-byte boundaries; others are copied first.
     Tensor rows_dy = dy, rows_codes = codes;
     if (dy.scalar_type() == ScalarType::BFloat16 && !on_16_bytes(dy, 2)) {
