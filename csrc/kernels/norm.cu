@@ -92,17 +92,16 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
                 }
             }
             if (p.keep == kKeepFp8) {
-                const int k = block_exponent(lanes_max(amax));
-                const float down = exp2_int(-k);
+                const BlockScale scale = block_scale(lanes_max(amax));
                 uint8_t *codes = p.codes + r * p.codes_stride;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t c = blk * kCheckpointBlock + i * 32 + lane;
                     if (c < p.width)
-                        codes[c] = uint8_t(to_e4m3x2(h[i] * down, 0.f));
+                        codes[c] = to_e4m3(h[i] * scale.down);
                 }
                 if (lane == 0)
-                    p.code_scales[r * blocks + blk] = exp2_int(k);
+                    p.code_scales[r * blocks + blk] = scale.up;
             }
         }
     }
@@ -196,6 +195,8 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     const uint8_t *w_at = static_cast<const uint8_t *>(p.weight) + share.chunk * Raw8<PARAM>::kBytes;
     const uint8_t *b_at = static_cast<const uint8_t *>(p.bias) + share.chunk * Raw8<PARAM>::kBytes;
     const uint32_t blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
+    uint8_t *code_at = p.codes + share.row * p.codes_stride + share.chunk * 8;
+    float *code_scale_at = p.code_scales + int64_t(share.row) * blocks + share.chunk / 16;
     const bool affine = p.weight != nullptr, shifted = p.bias != nullptr;
     for (uint32_t r = share.row; r < rows; r += share.step) {
         if (!mbar_wait(&s_full[share.group][slot], phase, kWaitNs)) {
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
                     // Finite, or NaN in all of a row: an infinity makes the mean NaN or infinite.
                     x[i][e] = mul2(add2(x[i][e], minus_shift), up);
                     if constexpr (FP8)
-                        amax = fmaxf(amax, fmaxf(fabsf(parts(x[i][e]).x), fabsf(parts(x[i][e]).y)));
+                        amax = largest3(amax, parts(x[i][e]).x, parts(x[i][e]).y);
                 }
                 if (affine) {
                     Pair v[4], w[4];
@@ -277,16 +278,19 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
                 }
             }
             if constexpr (FP8) {
-                const int k = block_exponent(lanes_max<16>(amax));
+                const BlockScale unit = block_scale(lanes_max<16>(amax));
                 if (there(i)) {
-                    const uint32_t c = share.chunk + i * 32;
-                    *reinterpret_cast<uint2 *>(p.codes + r * p.codes_stride + c * 8) = to_e4m3x8(x[i], exp2_int(-k));
+                    *reinterpret_cast<uint2 *>(code_at + i * 256) = to_e4m3x8(x[i], unit.down);
                     if (lane % 16 == 0)
-                        p.code_scales[int64_t(r) * blocks + c / 16] = exp2_int(k);
+                        code_scale_at[i * 2] = unit.up;
                 }
             }
         }
         y_at += y_step;
+        if constexpr (FP8) {
+            code_at += share.step * p.codes_stride;
+            code_scale_at += int64_t(share.step) * blocks;
+        }
     }
 }
 

@@ -72,25 +72,33 @@ __device__ __forceinline__ float finite_abs(float v) {
     return a <= FLT_MAX ? a : 0.f;
 }
 
-__device__ __forceinline__ int block_exponent(float amax) {
-    const uint32_t bits = __float_as_uint(amax);
-    const int k = int(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return amax == 0.f ? 0 : max(k, -126);
+struct BlockScale {
+    float up, down;  // 2^k and 2^-k
+};
+
+__device__ __forceinline__ BlockScale block_scale(float amax) {
+    // 2^k's bits: amax's exponent less 8, one more where its fraction is above .75
+    // (the addition then carries into the exponent).
+    const int bits = int((__float_as_uint(amax) + 0x1FFFFFu) & 0x7F800000u) - (8 << 23);
+    const uint32_t up = amax == 0.f ? 127u << 23 : uint32_t(max(bits, 1 << 23));
+    return {__uint_as_float(up), __uint_as_float((254u << 23) - up)};
 }
 
-__device__ __forceinline__ float exp2_int(int k) { return __uint_as_float(uint32_t(k + 127) << 23); }
-
-// Two codes (the first in the low byte) of values already divided by the scale.
-__device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
+// The code of a value already divided by its scale.
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
     // The conversion saturates infinities; here they have to stay visible.
-    const float nan = __uint_as_float(0x7FFFFFFFu);
-    a = fabsf(a) <= FLT_MAX ? a : nan;
-    b = fabsf(b) <= FLT_MAX ? b : nan;
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    return __nv_cvt_float_to_fp8(fabsf(v) <= FLT_MAX ? v : __uint_as_float(0x7FFFFFFFu), __NV_SATFINITE, __NV_E4M3);
 }
 
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two), __NV_E4M3)));
+}
+
+// The largest magnitude of three, NaN passed by.
+__device__ __forceinline__ float largest3(float a, float b, float c) {
+    float r;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 template <int LANES = 32> __device__ __forceinline__ float lanes_max(float v) {
