@@ -88,10 +88,54 @@ constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
 constexpr uint32_t kDyBytes = 4 * kDyChunk, kCodeBytes = 4 * kCodeChunk, kOperandBytes = 4 * kDyChunk;
 constexpr uint32_t kRingBytes = kLoadStages * (kDyBytes + kCodeBytes) + kOperandStages * kOperandBytes;
 constexpr uint32_t kSharedBytes = kRingBytes + 1024;  // + alignment of the swizzled tiles
-constexpr int kDecodeWarps = 8, kLoadWarp = 8, kMmaWarp = 9, kTensorThreads = 320;
+static_assert(kOperandStages == 2, "the decoders' turn is one bit");
+constexpr int kDecodeWarps = 16, kLoadWarp = 16, kScaleWarp = 17, kMmaWarp = 18, kTensorThreads = 19 * 32;
+constexpr uint32_t kBlocks = 3;              // 128-column blocks that a tile touches at most
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kStageRow = 66;           // floats per row of an epilogue tile
 constexpr uint64_t kWaitNs = 2000000000ull;  // far above any legal wait
+
+// How a row's 128-column block is decoded.  Four codes s eeee mmm become four
+// bf16 values by moving their bits to s 0000eeee mmm0000, the code's value
+// times 2^-120 (subnormal codes included), and one multiplication by scale *
+// 2^120: exact where the scale is a power of two up to 2^7.  Any other scale
+// (and a NaN code, whose bits would read as 480) takes a conversion by way of
+// fp32, rounded once.
+struct Decoder {
+    uint32_t factor;  // scale * 2^120 as two bf16, 0: by way of fp32
+    float scale;
+};
+__device__ __forceinline__ Decoder decoder_of(float scale) {
+    const uint32_t bits = __float_as_uint(scale);
+    const bool simple = (bits & 0x7FFFFFu) == 0 && bits >= 1u << 23 && bits <= (127u + 7) << 23;
+    return {simple ? __byte_perm(bits + (120u << 23), 0, 0x3232) : 0, scale};
+}
+
+// Words of a 16-code unit in which some byte is a NaN code have a bit of 0x80808080 set.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) { return (codes & 0x7F7F7F7Fu) + 0x01010101u; }
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Codes 0 and 2 of a word, then 1 and 3: pairs that lie sixteen bits apart need
+// no byte moves.  The columns of the product are put back in order where they
+// leave TMEM.
+__host__ __device__ constexpr uint32_t true_column(uint32_t c) {
+    return c % 4 == 1 ? c + 1 : c % 4 == 2 ? c - 1 : c;
+}
+__device__ __forceinline__ void decode4(uint32_t codes, uint32_t factor, uint32_t &even, uint32_t &odd) {
+    const uint32_t up = codes << 8;
+    even = mul_bf16x2((up & 0x80008000u) | (up >> 4 & 0x07F007F0u), factor);
+    odd = mul_bf16x2((codes & 0x80008000u) | (codes >> 4 & 0x07F007F0u), factor);
+}
+__device__ __forceinline__ void decode4_by_fp32(uint32_t codes, float scale, uint32_t &even, uint32_t &odd) {
+    const float2 a = from_e4m3x2(codes & 0xFFFFu), b = from_e4m3x2(codes >> 16);
+    even = to_bf16x2(a.x * scale, b.x * scale);
+    odd = to_bf16x2(a.y * scale, b.y * scale);
+}
 
 struct Shared {
     uint64_t loaded[kLoadStages], load_free[kLoadStages];
@@ -99,18 +143,27 @@ struct Shared {
     uint64_t done;
     uint32_t tmem;
     uint32_t failed;
+    Decoder decoders[kLoadStages][kBlocks][kSteps];
 };
 
-// Four codes as four bf16 values.
-__device__ __forceinline__ void decode4(uint32_t codes, float scale, uint32_t &low, uint32_t &high) {
-    const float2 a = from_e4m3x2(codes & 0xFFFFu), b = from_e4m3x2(codes >> 16);
-    low = to_bf16x2(a.x * scale, a.y * scale);
-    high = to_bf16x2(b.x * scale, b.y * scale);
+__device__ __forceinline__ Vec16 load_shared16(uint32_t at) {
+    Vec16 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 load_shared8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void store_shared16(uint32_t at, const Vec16 &v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 // One block: halves x 128 outputs by tile_k columns over one part of the rows.
-// Warp 8 copies tiles of dy and codes into a ring of three stages; warps 0-7
-// decode a stage's codes into one of two operand buffers; warp 9 issues the
+// Warp 16 copies tiles of dy and codes into a ring of three stages; warps 0-15
+// decode a stage's codes into one of two operand buffers, by the factors that
+// warp 17 makes of its scales; warp 18 issues the
 // MMAs of a stage for both halves, so each decoded value is used 256 times.
 // Accumulators fill TMEM (2 x 256 columns).
 __global__ void __launch_bounds__(kTensorThreads, 1)
@@ -132,7 +185,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kLoadStages; ++i) {
-            mbar_init(&s.loaded[i], 1);
+            mbar_init(&s.loaded[i], 2);  // the copies and the decoders
             mbar_init(&s.load_free[i], kDecodeWarps + 1);
         }
         for (int i = 0; i < kOperandStages; ++i) {
@@ -197,58 +250,101 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
             }
             mma_commit(&s.done);
         }
-    } else {
-        // A warp takes 32 rows and every fourth 16-byte unit of them: eight lanes
-        // of one shared-memory phase are eight rows of one unit, which both
-        // swizzles spread over all banks.
-        const uint32_t row = warp % 2 * 32 + lane, units = (columns + 15) / 16;
+    } else if (warp == kScaleWarp) {
+        // Lane l: rows l and l + 32 of a stage, one stage of loads ahead.
         const uint32_t block0 = k0 / kCheckpointBlock;
-        const uint32_t blocks = (k0 + columns - 1) / kCheckpointBlock - block0 + 1;  // at most 3
+        const uint32_t blocks = (k0 + columns - 1) / kCheckpointBlock - block0 + 1;
         const float *scales = p.scales + block0 * p.scale_col_stride;
-        float next[3];
-        auto load_scales = [&](uint32_t i) {
-            const int64_t m = int64_t((first + i) % plane_steps) * kSteps + row;
+        float next[2][kBlocks];
+        auto load = [&](uint32_t i) {
+            const int64_t m = int64_t((first + i) % plane_steps) * kSteps + lane;
 #pragma unroll
-            for (uint32_t b = 0; b < 3; ++b)
-                next[b] = m < p.rows && b < blocks ? __ldg(scales + m * p.scale_row_stride + b * p.scale_col_stride) : 1.f;
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t b = 0; b < kBlocks; ++b)
+                    next[h][b] = m + h * 32 < p.rows && b < blocks
+                                     ? __ldg(scales + (m + h * 32) * p.scale_row_stride + b * p.scale_col_stride)
+                                     : 1.f;
         };
-        load_scales(0);
+        load(0);
         for (uint32_t i = 0; i < steps; ++i) {
-            const uint32_t at = i % kLoadStages, to = i % kOperandStages;
-            const float scale0 = next[0], scale1 = next[1], scale2 = next[2];
-            if (i + 1 < steps)
-                load_scales(i + 1);
-            ok = mbar_wait(&s.loaded[at], i / kLoadStages & 1, kWaitNs) &&
-                 mbar_wait(&s.operand_free[to], (i / kOperandStages & 1) ^ 1, kWaitNs);
+            const uint32_t at = i % kLoadStages;
+            ok = mbar_wait(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok)
                 break;
-            const uint8_t *codes = code_tiles + at * kCodeBytes + row * 64;
-            uint8_t *operand = operands + to * kOperandBytes + row * 128;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t u = warp / 2 + j * 4;
-                if (u < units) {
-                    const uint32_t b = (k0 + u * 16) / kCheckpointBlock - block0;
-                    const float scale = b == 0 ? scale0 : b == 1 ? scale1 : scale2;
-                    const Vec16 v = ld_shared_v4(codes + u / 4 * kCodeChunk + ((u % 4 ^ (row >> 1 & 3)) << 4));
-                    uint4 x, y;
-                    decode4(v.x, scale, x.x, x.y);
-                    decode4(v.y, scale, x.z, x.w);
-                    decode4(v.z, scale, y.x, y.y);
-                    decode4(v.w, scale, y.z, y.w);
-                    uint8_t *out = operand + u / 4 * kDyChunk;
-                    const uint32_t chunk = u % 4 * 2;
-                    *reinterpret_cast<uint4 *>(out + ((chunk ^ (row & 7)) << 4)) = x;
-                    *reinterpret_cast<uint4 *>(out + ((chunk + 1 ^ (row & 7)) << 4)) = y;
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t b = 0; b < kBlocks; ++b)
+                    s.decoders[at][b][lane + h * 32] = decoder_of(next[h][b]);
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&s.loaded[at]);
+            if (i + 1 < steps)
+                load(i + 1);
+        }
+    } else {
+        // A warp takes 32 rows and every eighth 16-byte unit of them: eight lanes
+        // of one shared-memory phase are eight rows of one unit, which both
+        // swizzles spread over all banks.  Nothing but the stage changes from
+        // one to the next.
+        constexpr int kUnits = 2;
+        const uint32_t row = warp % 2 * 32 + lane, units = (columns + 15) / 16;
+        uint32_t from[kUnits], to_low[kUnits], to_high[kUnits], decoder[kUnits];
+#pragma unroll
+        for (uint32_t j = 0; j < kUnits; ++j) {
+            const uint32_t u = warp / 2 + j * 8, chunk = u % 4 * 2;
+            from[j] = smem_addr(code_tiles) + u / 4 * kCodeChunk + row * 64 + ((u % 4 ^ (row >> 1 & 3)) << 4);
+            to_low[j] = smem_addr(operands) + u / 4 * kDyChunk + row * 128 + ((chunk ^ (row & 7)) << 4);
+            to_high[j] = smem_addr(operands) + u / 4 * kDyChunk + row * 128 + ((chunk + 1 ^ (row & 7)) << 4);
+            const uint32_t b = (k0 + u * 16) / kCheckpointBlock - k0 / kCheckpointBlock;
+            decoder[j] = smem_addr(&s.decoders[0][min(b, kBlocks - 1)][row]);
+        }
+        uint32_t at = 0, load_phase = 0, to = 0, operand_phase = 1;
+        for (uint32_t i = 0; i < steps; ++i) {
+            ok = mbar_wait(&s.loaded[at], load_phase, kWaitNs) && mbar_wait(&s.operand_free[to], operand_phase, kWaitNs);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok)
+                break;
+            Vec16 v[kUnits];
+            uint2 d[kUnits];
+#pragma unroll
+            for (uint32_t j = 0; j < kUnits; ++j)
+                if (warp / 2 + j * 8 < units) {
+                    v[j] = load_shared16(from[j] + at * kCodeBytes);
+                    d[j] = load_shared8(decoder[j] + at * uint32_t(sizeof(s.decoders[0])));
                 }
-            }
+#pragma unroll
+            for (uint32_t j = 0; j < kUnits; ++j)
+                if (warp / 2 + j * 8 < units) {
+                    const uint32_t nan = (nan_bytes(v[j].x) | nan_bytes(v[j].y) | nan_bytes(v[j].z) | nan_bytes(v[j].w)) & 0x80808080u;
+                    Vec16 x, y;
+                    if (d[j].x != 0 && nan == 0) {
+                        decode4(v[j].x, d[j].x, x.x, x.y);
+                        decode4(v[j].y, d[j].x, x.z, x.w);
+                        decode4(v[j].z, d[j].x, y.x, y.y);
+                        decode4(v[j].w, d[j].x, y.z, y.w);
+                    } else {
+                        const float scale = __uint_as_float(d[j].y);
+                        decode4_by_fp32(v[j].x, scale, x.x, x.y);
+                        decode4_by_fp32(v[j].y, scale, x.z, x.w);
+                        decode4_by_fp32(v[j].z, scale, y.x, y.y);
+                        decode4_by_fp32(v[j].w, scale, y.z, y.w);
+                    }
+                    store_shared16(to_low[j] + to * kOperandBytes, x);
+                    store_shared16(to_high[j] + to * kOperandBytes, y);
+                }
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&s.decoded[to]);
                 mbar_arrive(&s.load_free[at]);
             }
+            at = at + 1 == kLoadStages ? 0 : at + 1;
+            load_phase ^= at == 0 ? 1 : 0;
+            to ^= 1;
+            operand_phase ^= to == 0 ? 1 : 0;
         }
     }
     if (!ok)
@@ -263,10 +359,10 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
             // rows of the tile in shared memory (the ring is free), then lane =
             // column, so that rows are stored whole.
             float *tile = reinterpret_cast<float *>(ring) + warp * 32 * kStageRow;
-            const uint32_t half = p.halves == 2 ? warp / 4 : 0, row0 = warp % 4 * 32;
-            const uint32_t chunk_step = p.halves == 2 ? 64 : 128;
+            const uint32_t half = p.halves == 2 ? warp / 4 % 2 : 0, row0 = warp % 4 * 32;
+            const uint32_t chunk_step = p.halves == 2 ? 128 : 256;
             const bool direct = p.parts == 1;
-            for (uint32_t c0 = p.halves == 2 ? 0 : warp / 4 * 64; c0 < columns; c0 += chunk_step) {
+            for (uint32_t c0 = (p.halves == 2 ? warp / 8 : warp / 4) * 64; c0 < columns; c0 += chunk_step) {
                 uint32_t v[2][32];
                 const uint32_t address = tmem + (row0 << 16) + half * 256 + c0;
                 tmem_load32(address, v[0]);
@@ -276,7 +372,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
                 __syncwarp();
 #pragma unroll
                 for (int c = 0; c < 64; ++c)
-                    tile[lane * kStageRow + c] = __uint_as_float(v[c / 32][c % 32]);
+                    tile[lane * kStageRow + true_column(c)] = __uint_as_float(v[c / 32][c % 32]);
                 __syncwarp();
                 const uint32_t c = c0 + lane * 2, k = k0 + c;
                 const bool there[2] = {c < columns, c + 1 < columns};
