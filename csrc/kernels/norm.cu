@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     float *code_scale_at = p.code_scales + int64_t(share.row) * blocks + share.chunk / 16;
     const bool affine = p.weight != nullptr, shifted = p.bias != nullptr;
     for (uint32_t r = share.row; r < rows; r += share.step) {
-        if (!mbar_wait(&s_full[share.group][slot], phase, kWaitNs)) {
+        if (!mbar_wait_often(&s_full[share.group][slot], phase, kWaitNs)) {
             st_release_sys_u32(p.fault, kPipelineTimeout);
             return;
         }
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
         }
         if (r + share.step < rows)
             load_stats(r + share.step);
-        if (!mbar_wait(&s_full[share.group][slot], phase, kWaitNs)) {
+        if (!mbar_wait_often(&s_full[share.group][slot], phase, kWaitNs)) {
             st_release_sys_u32(p.fault, kPipelineTimeout);
             return;
         }

@@ -228,6 +228,28 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64
     return true;
 }
 
+// Polls until `done`; false after `timeout_ns` (or as many polls).  The timer is
+// read once in 256 polls: a read takes as long as many of them, and a waiter
+// in the middle of one sees its barrier late.
+template <class Done> __device__ __forceinline__ bool mbar_poll(uint64_t timeout_ns, Done done) {
+    uint64_t start = 0;
+    for (uint64_t polls = 1; !done(); ++polls) {
+        if (polls % 256 != 0)
+            continue;
+        const uint64_t now = global_timer_ns();
+        if (start == 0)
+            start = now;
+        if (now - start > timeout_ns || polls > timeout_ns)
+            return false;
+    }
+    return true;
+}
+
+// mbar_wait for waits on the critical path of a pipeline.
+__device__ __forceinline__ bool mbar_wait_often(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
+    return mbar_poll(timeout_ns, [&] { return mbar_try_wait(bar, parity); });
+}
+
 // Non-multicast bulk copy global -> this CTA's shared memory, completing
 // `bytes` of transaction count on `bar`.  Source and size are 16-byte multiples.
 __device__ __forceinline__ void bulk_load(void *dst_smem, const void *src, uint32_t bytes, uint64_t *bar) {

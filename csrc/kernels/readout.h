@@ -91,8 +91,8 @@ struct WeightGradParams {
     uint32_t *fault;                      // host-mapped: set when a wait ran out
     int64_t rows, dy_stride, codes_stride, scale_row_stride, scale_col_stride, plane_stride;
     uint32_t width, out, type, param_type, out_type, sum_rows;
-    // The plan (plan_weight_grad): dy as `planes` bf16 terms; blocks of `halves`
-    // x 128 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64.
+    // The plan (plan_weight_grad): dy as `planes` bf16 terms; pairs of blocks for
+    // `halves` x 256 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64.
     uint32_t planes, halves, tile_k, tiles_k, tiles_o, parts, part_steps;
 };
 

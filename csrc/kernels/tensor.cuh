@@ -26,16 +26,21 @@ __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap *map) {
 // Plain shared-memory stores before it are visible to the async proxy after.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// TMEM: `columns` columns of 128 lanes x 32 bits; the address lands in `*slot`.
+// The MMAs here run on a pair of SMs (a cluster of two blocks, the even one of
+// them the leader): each block holds half of the rows of A and of the result,
+// and half of the columns of B.
+
+// TMEM: `columns` columns of 128 lanes x 32 bits in both blocks of the pair (a
+// warp of each calls it); the address lands in `*slot`.
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)),
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)),
                  "r"(columns)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
 }
 
 __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
 }
 
 // 32 consecutive columns of this warp's 32 lanes (lane = row).  The values are
@@ -59,10 +64,37 @@ __device__ __forceinline__ void tensor_fence_before() {
 }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// `bar` gets one arrival when every MMA this thread issued so far is done.
+// `bar` of both blocks gets one arrival when every MMA this thread issued so far is done.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_addr(bar)),
+                 "h"(uint16_t(3))
                  : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// All threads of the pair (stores before it are visible after it).
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The leader's barrier at the place of this block's `bar`.
+__device__ __forceinline__ uint32_t leader_barrier(const uint64_t *bar) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_addr(bar)));
+    return at;
+}
+// Arrives there.  What it announces are operands for the pair's MMAs, which this
+// SM's own tensor core reads: fence_async_shared before it orders them, and no
+// thread of the other block reads them.  (A release at cluster scope took a
+// third of a stage's time.)
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Shared-memory operand stored with its non-reduction dimension contiguous and
@@ -74,15 +106,15 @@ __device__ __forceinline__ uint64_t mma_operand(const void *smem, uint32_t chunk
            (uint64_t(step_stride >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
-// bf16 x bf16 -> fp32, both operands transposed as above, 128 x n outputs.
+// bf16 x bf16 -> fp32, both operands transposed as above, 256 x n outputs.
 __device__ __forceinline__ uint32_t mma_shape_bf16(uint32_t n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
 
-// One 128 x n x 16 step into TMEM at `d`; `add` 0 overwrites.
+// One 256 x n x 16 step of the pair into TMEM at `d`; `add` 0 overwrites.  The leader issues it.
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
                  "l"(a), "l"(b), "r"(shape), "r"(add)
                  : "memory");
 }

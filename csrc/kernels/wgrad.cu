@@ -82,17 +82,17 @@ __global__ void __launch_bounds__(kThreads) split_dy(const __grid_constant__ Wei
 
 // ---------------------------------------------------------------- the product
 constexpr uint32_t kSteps = 64;              // rows per stage
-constexpr int kLoadStages = 3, kOperandStages = 2;
+constexpr int kLoadStages = 4, kOperandStages = 3;
 constexpr uint32_t kDyChunk = kSteps * 128;  // 64 columns of dy (bf16)
 constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
-constexpr uint32_t kDyBytes = 4 * kDyChunk, kCodeBytes = 4 * kCodeChunk, kOperandBytes = 4 * kDyChunk;
+// A block's share of a pair's stage: 2 x 128 outputs, 128 columns.
+constexpr uint32_t kDyBytes = 4 * kDyChunk, kCodeBytes = 2 * kCodeChunk, kOperandBytes = 2 * kDyChunk;
 constexpr uint32_t kRingBytes = kLoadStages * (kDyBytes + kCodeBytes) + kOperandStages * kOperandBytes;
 constexpr uint32_t kSharedBytes = kRingBytes + 1024;  // + alignment of the swizzled tiles
-static_assert(kOperandStages == 2, "the decoders' turn is one bit");
-constexpr int kDecodeWarps = 16, kLoadWarp = 16, kScaleWarp = 17, kMmaWarp = 18, kTensorThreads = 19 * 32;
-constexpr uint32_t kBlocks = 3;              // 128-column blocks that a tile touches at most
+constexpr int kDecodeWarps = 8, kLoadWarp = 8, kScaleWarp = 9, kMmaWarp = 10, kTensorThreads = 11 * 32;
+constexpr uint32_t kBlocks = 2;              // 128-column blocks that a block's share touches at most
 constexpr uint32_t kTmemColumns = 512;
-constexpr uint32_t kStageRow = 66;           // floats per row of an epilogue tile
+constexpr uint32_t kStageRow = 68;           // floats per row of an epilogue tile: 16-byte stores meet all banks
 constexpr uint64_t kWaitNs = 2000000000ull;  // far above any legal wait
 
 // How a row's 128-column block is decoded.  Four codes s eeee mmm become four
@@ -122,10 +122,7 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 
 // Codes 0 and 2 of a word, then 1 and 3: pairs that lie sixteen bits apart need
 // no byte moves.  The columns of the product are put back in order where they
-// leave TMEM.
-__host__ __device__ constexpr uint32_t true_column(uint32_t c) {
-    return c % 4 == 1 ? c + 1 : c % 4 == 2 ? c - 1 : c;
-}
+// leave TMEM (store_tile).
 __device__ __forceinline__ void decode4(uint32_t codes, uint32_t factor, uint32_t &even, uint32_t &odd) {
     const uint32_t up = codes << 8;
     even = mul_bf16x2((up & 0x80008000u) | (up >> 4 & 0x07F007F0u), factor);
@@ -160,13 +157,90 @@ __device__ __forceinline__ void store_shared16(uint32_t at, const Vec16 &v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// One block: halves x 128 outputs by tile_k columns over one part of the rows.
-// Warp 16 copies tiles of dy and codes into a ring of three stages; warps 0-15
-// decode a stage's codes into one of two operand buffers, by the factors that
-// warp 17 makes of its scales; warp 18 issues the
-// MMAs of a stage for both halves, so each decoded value is used 256 times.
-// Accumulators fill TMEM (2 x 256 columns).
-__global__ void __launch_bounds__(kTensorThreads, 1)
+// A block's accumulators to memory: a warp turns 32 rows x 64 columns at a time
+// by way of its part `tile` of the ring, which is free by then (TMEM gives a
+// lane a row; rows are to be stored whole).
+__device__ __forceinline__ void store_tile(const WeightGradParams &p, uint32_t tmem, float *tile, uint32_t o0, uint32_t k0,
+                                           uint32_t part) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, columns = min(p.tile_k, p.width - k0);
+    const uint32_t half = p.halves == 2 ? warp / 4 : 0, row0 = warp % 4 * 32;
+    const uint32_t o_first = o0 + half * 256 + row0;
+    if (o_first >= p.out)
+        return;
+    const uint32_t o_rows = min(32u, p.out - o_first);
+    const bool direct = p.parts == 1, weighted = direct && p.norm_weight != nullptr, shifted = direct && p.norm_bias != nullptr;
+    const float row_sum = shifted && lane < o_rows ? p.dy_sums[o_first + lane] : 0.f;
+    const uint32_t out_bytes = direct ? element_bytes(p.out_type) : 4;
+    uint8_t *out = direct ? static_cast<uint8_t *>(p.dweight)
+                          : reinterpret_cast<uint8_t *>(p.dw_parts + int64_t(part) * p.out * p.width);
+    const uint32_t out_type = direct ? p.out_type : uint32_t(kFp32);
+    // Two columns of a lane in one store: both rows and pairs start on its boundary.
+    const bool pairs = p.width % 2 == 0;
+    for (uint32_t c0 = p.halves == 2 ? 0 : warp / 4 * 64; c0 < columns; c0 += p.halves == 2 ? 64 : 128) {
+        uint32_t v[2][32];
+        const uint32_t address = tmem + (row0 << 16) + half * 256 + c0;
+        tmem_load32(address, v[0]);
+        tmem_load32(address + 32, v[1]);
+        const uint32_t c = c0 + lane * 2, k = k0 + c;
+        const bool there0 = c < columns, there1 = c + 1 < columns;
+        float w0 = 1.f, w1 = 1.f, b0 = 0.f, b1 = 0.f;
+        if (weighted) {
+            w0 = there0 ? load_param(p.norm_weight, p.param_type, k) : 0.f;
+            w1 = there1 ? load_param(p.norm_weight, p.param_type, k + 1) : 0.f;
+        }
+        if (shifted) {
+            b0 = there0 ? load_param(p.norm_bias, p.param_type, k) : 0.f;
+            b1 = there1 ? load_param(p.norm_bias, p.param_type, k + 1) : 0.f;
+        }
+        tmem_wait_loads();
+        __syncwarp();  // the tile's last rows have been read
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const uint32_t *f = &v[q / 8][q % 8 * 4];  // in the decoders' order: columns 0, 2, 1, 3
+            *reinterpret_cast<uint4 *>(tile + lane * kStageRow + q * 4) = make_uint4(f[0], f[2], f[1], f[3]);
+        }
+        __syncwarp();
+        uint8_t *at = out + (int64_t(o_first) * p.width + k) * out_bytes;
+        const int64_t row_bytes = int64_t(p.width) * out_bytes;
+#pragma unroll 8
+        for (uint32_t r = 0; r < o_rows; ++r, at += row_bytes) {
+            float2 x = *reinterpret_cast<const float2 *>(tile + r * kStageRow + lane * 2);
+            if (weighted) {
+                x.x *= w0;
+                x.y *= w1;
+            }
+            if (shifted) {
+                const float sum = __shfl_sync(0xFFFFFFFFu, row_sum, r);
+                x.x += b0 * sum;
+                x.y += b1 * sum;
+            }
+            if (pairs && there1) {
+                if (out_type == kFp32)
+                    *reinterpret_cast<float2 *>(at) = x;
+                else
+                    *reinterpret_cast<uint32_t *>(at) = out_type == kBf16 ? to_bf16x2(x.x, x.y) : to_fp16x2(x.x, x.y);
+            } else {
+                if (there0)
+                    store_param(at, out_type, 0, x.x);
+                if (there1)
+                    store_param(at, out_type, 1, x.y);
+            }
+        }
+    }
+}
+
+// A pair of blocks: halves x 256 outputs by tile_k columns over one part of the
+// rows, by 256 x n x 16 MMAs on both SMs.  Each block brings its 128 rows of a
+// half's dy and decodes half of the columns; the tensor cores read the other
+// half from the other block, and each decoded value is used 512 times.  With
+// one SM on its own (256 x 256 outputs) shared memory was the bound: 192 KB
+// moved through it per 1024 cycles of MMAs against 128 KB here.
+//
+// Warp 8 copies tiles of dy and codes into a ring of four stages; warps 0-7
+// decode a stage's codes into one of three operand buffers, by the factors
+// that warp 9 makes of its scales; the leader's warp 10 issues the MMAs of a
+// stage for both halves.  Accumulators fill TMEM (2 x 256 columns).
+__global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     weight_grad_tensor(const __grid_constant__ WeightGradParams p, const __grid_constant__ CUtensorMap dy_map,
                        const __grid_constant__ CUtensorMap code_map) {
     extern __shared__ uint8_t s_raw[];
@@ -174,14 +248,16 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
     uint8_t *ring = s_raw + ((1024u - (smem_addr(s_raw) & 1023u)) & 1023u);
     uint8_t *dy_tiles = ring, *code_tiles = ring + kLoadStages * kDyBytes,
             *operands = code_tiles + kLoadStages * kCodeBytes;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t o0 = blockIdx.x % p.tiles_o * (p.halves * 128);
-    const uint32_t k0 = blockIdx.x / p.tiles_o % p.tiles_k * p.tile_k;
-    const uint32_t part = blockIdx.x / (p.tiles_o * p.tiles_k);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = cluster_rank();
+    const uint32_t tile = blockIdx.x / 2, share = p.tile_k / 2;
+    const uint32_t o0 = tile % p.tiles_o * (p.halves * 256) + rank * 128;  // half h: o0 + h * 256
+    const uint32_t tile_k0 = tile / p.tiles_o % p.tiles_k * p.tile_k;
+    const uint32_t k0 = tile_k0 + rank * share;                            // this block's columns to decode
+    const uint32_t part = tile / (p.tiles_o * p.tiles_k);
     const uint32_t plane_steps = uint32_t((p.rows + kSteps - 1) / kSteps);
     const uint32_t first = part * p.part_steps;
     const uint32_t steps = min(p.part_steps, plane_steps * p.planes - first);
-    const uint32_t columns = min(p.tile_k, p.width - k0);
+    const uint32_t columns = k0 < p.width ? min(share, p.width - k0) : 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kLoadStages; ++i) {
@@ -189,7 +265,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
             mbar_init(&s.load_free[i], kDecodeWarps + 1);
         }
         for (int i = 0; i < kOperandStages; ++i) {
-            mbar_init(&s.decoded[i], kDecodeWarps);
+            mbar_init(&s.decoded[i], 2 * kDecodeWarps);
             mbar_init(&s.operand_free[i], 1);
         }
         mbar_init(&s.done, 1);
@@ -200,6 +276,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         tmem_alloc(&s.tmem, kTmemColumns);
     tensor_fence_before();
     __syncthreads();
+    cluster_sync();  // the other block's barriers are there
     tensor_fence_after();
     const uint32_t tmem = s.tmem;
 
@@ -208,33 +285,36 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         if (lane == 0) {
             prefetch_tensor_map(&dy_map);
             prefetch_tensor_map(&code_map);
-            const uint32_t dy_chunks = (min(p.halves * 128, p.out - o0) + 63) / 64, code_chunks = (columns + 63) / 64;
+            uint32_t dy_chunks = 0;
+            for (uint32_t c = 0; c < p.halves * 2; ++c)
+                dy_chunks += o0 + c / 2 * 256 + c % 2 * 64 < p.out;  // the first ones: outputs ascend
+            const uint32_t code_chunks = (columns + 63) / 64;
             uint32_t i = 0;
             for (; ok && i < steps; ++i) {
                 const uint32_t at = i % kLoadStages, g = first + i;
-                ok = mbar_wait(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
+                ok = mbar_wait_often(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
                 if (!ok)
                     break;
                 const int m = int(g % plane_steps * kSteps), plane = int(g / plane_steps);
                 mbar_arrive_expect_tx(&s.loaded[at], dy_chunks * kDyChunk + code_chunks * kCodeChunk);
                 for (uint32_t c = 0; c < dy_chunks; ++c)
-                    tensor_load_3d(dy_tiles + at * kDyBytes + c * kDyChunk, &dy_map, int(o0 + c * 64), m, plane,
-                                   &s.loaded[at]);
+                    tensor_load_3d(dy_tiles + at * kDyBytes + c * kDyChunk, &dy_map, int(o0 + c / 2 * 256 + c % 2 * 64), m,
+                                   plane, &s.loaded[at]);
                 for (uint32_t c = 0; c < code_chunks; ++c)
                     tensor_load_3d(code_tiles + at * kCodeBytes + c * kCodeChunk, &code_map, int(k0 + c * 64), m, 0,
                                    &s.loaded[at]);
             }
             if (!ok)  // let the copies in flight land before the block goes
                 for (uint32_t j = i > kLoadStages ? i - kLoadStages : 0; j < i; ++j)
-                    mbar_wait(&s.loaded[j % kLoadStages], j / kLoadStages & 1, kWaitNs);
+                    mbar_wait_often(&s.loaded[j % kLoadStages], j / kLoadStages & 1, kWaitNs);
         }
     } else if (warp == kMmaWarp) {
-        if (lane == 0) {
+        if (rank == 0 && lane == 0) {
             const uint32_t shape = mma_shape_bf16(p.tile_k);
+            uint32_t at = 0, to = 0, phase = 0;
             for (uint32_t i = 0; i < steps; ++i) {
-                const uint32_t at = i % kLoadStages, to = i % kOperandStages;
-                ok = mbar_wait(&s.loaded[at], i / kLoadStages & 1, kWaitNs) &&
-                     mbar_wait(&s.decoded[to], i / kOperandStages & 1, kWaitNs);
+                // Both blocks' decoders have seen their dy tiles land too.
+                ok = mbar_wait_often(&s.decoded[to], phase, kWaitNs);
                 if (!ok)
                     break;
                 tensor_fence_after();
@@ -247,45 +327,55 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
                                  (i | j) != 0);
                 mma_commit(&s.load_free[at]);
                 mma_commit(&s.operand_free[to]);
+                at = at + 1 == kLoadStages ? 0 : at + 1;
+                to = to + 1 == kOperandStages ? 0 : to + 1;
+                phase ^= to == 0 ? 1 : 0;
             }
             mma_commit(&s.done);
         }
     } else if (warp == kScaleWarp) {
-        // Lane l: rows l and l + 32 of a stage, one stage of loads ahead.
+        // Lane l: rows l and l + 32 of a stage.  Loads are kAhead stages ahead: one
+        // stage ahead, their latency was the time of a stage.
+        constexpr uint32_t kAhead = 8;
         const uint32_t block0 = k0 / kCheckpointBlock;
-        const uint32_t blocks = (k0 + columns - 1) / kCheckpointBlock - block0 + 1;
+        const uint32_t blocks = columns == 0 ? 0 : (k0 + columns - 1) / kCheckpointBlock - block0 + 1;
         const float *scales = p.scales + block0 * p.scale_col_stride;
-        float next[2][kBlocks];
-        auto load = [&](uint32_t i) {
+        float next[kAhead][2][kBlocks];
+        auto load = [&](uint32_t i, float (&to)[2][kBlocks]) {
             const int64_t m = int64_t((first + i) % plane_steps) * kSteps + lane;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
                 for (uint32_t b = 0; b < kBlocks; ++b)
-                    next[h][b] = m + h * 32 < p.rows && b < blocks
-                                     ? __ldg(scales + (m + h * 32) * p.scale_row_stride + b * p.scale_col_stride)
-                                     : 1.f;
+                    to[h][b] = i < steps && m + h * 32 < p.rows && b < blocks
+                                   ? __ldg(scales + (m + h * 32) * p.scale_row_stride + b * p.scale_col_stride)
+                                   : 1.f;
         };
-        load(0);
-        for (uint32_t i = 0; i < steps; ++i) {
-            const uint32_t at = i % kLoadStages;
-            ok = mbar_wait(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok)
-                break;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
+        for (uint32_t a = 0; a < kAhead; ++a)
+            load(a, next[a]);
+        for (uint32_t i0 = 0; ok && i0 < steps; i0 += kAhead)
 #pragma unroll
-                for (uint32_t b = 0; b < kBlocks; ++b)
-                    s.decoders[at][b][lane + h * 32] = decoder_of(next[h][b]);
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&s.loaded[at]);
-            if (i + 1 < steps)
-                load(i + 1);
-        }
+            for (uint32_t a = 0; a < kAhead; ++a) {
+                const uint32_t i = i0 + a, at = i % kLoadStages;
+                if (i >= steps)
+                    break;
+                ok = mbar_wait_often(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok)
+                    break;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t b = 0; b < kBlocks; ++b)
+                        s.decoders[at][b][lane + h * 32] = decoder_of(next[a][h][b]);
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&s.loaded[at]);
+                load(i + kAhead, next[a]);
+            }
     } else {
-        // A warp takes 32 rows and every eighth 16-byte unit of them: eight lanes
+        // A warp takes 32 rows and every fourth 16-byte unit of them: eight lanes
         // of one shared-memory phase are eight rows of one unit, which both
         // swizzles spread over all banks.  Nothing but the stage changes from
         // one to the next.
@@ -294,30 +384,32 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         uint32_t from[kUnits], to_low[kUnits], to_high[kUnits], decoder[kUnits];
 #pragma unroll
         for (uint32_t j = 0; j < kUnits; ++j) {
-            const uint32_t u = warp / 2 + j * 8, chunk = u % 4 * 2;
+            const uint32_t u = warp / 2 + j * 4, chunk = u % 4 * 2;
             from[j] = smem_addr(code_tiles) + u / 4 * kCodeChunk + row * 64 + ((u % 4 ^ (row >> 1 & 3)) << 4);
             to_low[j] = smem_addr(operands) + u / 4 * kDyChunk + row * 128 + ((chunk ^ (row & 7)) << 4);
             to_high[j] = smem_addr(operands) + u / 4 * kDyChunk + row * 128 + ((chunk + 1 ^ (row & 7)) << 4);
             const uint32_t b = (k0 + u * 16) / kCheckpointBlock - k0 / kCheckpointBlock;
             decoder[j] = smem_addr(&s.decoders[0][min(b, kBlocks - 1)][row]);
         }
+        const uint32_t leader = leader_barrier(&s.decoded[0]);
         uint32_t at = 0, load_phase = 0, to = 0, operand_phase = 1;
         for (uint32_t i = 0; i < steps; ++i) {
-            ok = mbar_wait(&s.loaded[at], load_phase, kWaitNs) && mbar_wait(&s.operand_free[to], operand_phase, kWaitNs);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok)
-                break;
+            ok = mbar_wait_often(&s.loaded[at], load_phase, kWaitNs);
             Vec16 v[kUnits];
             uint2 d[kUnits];
 #pragma unroll
             for (uint32_t j = 0; j < kUnits; ++j)
-                if (warp / 2 + j * 8 < units) {
+                if (warp / 2 + j * 4 < units) {
                     v[j] = load_shared16(from[j] + at * kCodeBytes);
                     d[j] = load_shared8(decoder[j] + at * uint32_t(sizeof(s.decoders[0])));
                 }
+            ok = ok && mbar_wait_often(&s.operand_free[to], operand_phase, kWaitNs);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok)
+                break;
 #pragma unroll
             for (uint32_t j = 0; j < kUnits; ++j)
-                if (warp / 2 + j * 8 < units) {
+                if (warp / 2 + j * 4 < units) {
                     const uint32_t nan = (nan_bytes(v[j].x) | nan_bytes(v[j].y) | nan_bytes(v[j].z) | nan_bytes(v[j].w)) & 0x80808080u;
                     Vec16 x, y;
                     if (d[j].x != 0 && nan == 0) {
@@ -338,12 +430,12 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&s.decoded[to]);
+                mbar_arrive_leader(leader + to * 8);
                 mbar_arrive(&s.load_free[at]);
             }
             at = at + 1 == kLoadStages ? 0 : at + 1;
             load_phase ^= at == 0 ? 1 : 0;
-            to ^= 1;
+            to = to + 1 == kOperandStages ? 0 : to + 1;
             operand_phase ^= to == 0 ? 1 : 0;
         }
     }
@@ -351,84 +443,23 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         s.failed = 1;
     __syncthreads();
     if (warp < kDecodeWarps) {
-        ok = mbar_wait(&s.done, 0, kWaitNs);
+        ok = mbar_wait_often(&s.done, 0, kWaitNs);
         ok = __all_sync(0xFFFFFFFFu, ok) && s.failed == 0;
         tensor_fence_after();
-        if (ok) {
-            // A warp turns 32 rows x 64 columns at a time: TMEM lane = row, then
-            // rows of the tile in shared memory (the ring is free), then lane =
-            // column, so that rows are stored whole.
-            float *tile = reinterpret_cast<float *>(ring) + warp * 32 * kStageRow;
-            const uint32_t half = p.halves == 2 ? warp / 4 % 2 : 0, row0 = warp % 4 * 32;
-            const uint32_t chunk_step = p.halves == 2 ? 128 : 256;
-            const bool direct = p.parts == 1;
-            for (uint32_t c0 = (p.halves == 2 ? warp / 8 : warp / 4) * 64; c0 < columns; c0 += chunk_step) {
-                uint32_t v[2][32];
-                const uint32_t address = tmem + (row0 << 16) + half * 256 + c0;
-                tmem_load32(address, v[0]);
-                if (c0 + 32 < columns)
-                    tmem_load32(address + 32, v[1]);
-                tmem_wait_loads();
-                __syncwarp();
-#pragma unroll
-                for (int c = 0; c < 64; ++c)
-                    tile[lane * kStageRow + true_column(c)] = __uint_as_float(v[c / 32][c % 32]);
-                __syncwarp();
-                const uint32_t c = c0 + lane * 2, k = k0 + c;
-                const bool there[2] = {c < columns, c + 1 < columns};
-                float w[2] = {1.f, 1.f}, b[2] = {0.f, 0.f};
-                for (int e = 0; e < 2; ++e)
-                    if (direct && there[e]) {
-                        if (p.norm_weight != nullptr)
-                            w[e] = load_param(p.norm_weight, p.param_type, k + e);
-                        if (p.norm_bias != nullptr)
-                            b[e] = load_param(p.norm_bias, p.param_type, k + e);
-                    }
-                for (uint32_t r = 0; r < 32; ++r) {
-                    const uint32_t o = o0 + half * 128 + row0 + r;
-                    if (o >= p.out)
-                        break;
-                    float2 x = *reinterpret_cast<const float2 *>(tile + r * kStageRow + lane * 2);
-                    const int64_t at = int64_t(o) * p.width + k;
-                    if (!direct) {
-                        float *to = p.dw_parts + int64_t(part) * p.out * p.width + at;
-                        if (there[0])
-                            to[0] = x.x;
-                        if (there[1])
-                            to[1] = x.y;
-                        continue;
-                    }
-                    if (p.norm_weight != nullptr) {
-                        x.x *= w[0];
-                        x.y *= w[1];
-                    }
-                    if (p.norm_bias != nullptr) {
-                        const float sum = p.dy_sums[o];
-                        x.x += b[0] * sum;
-                        x.y += b[1] * sum;
-                    }
-                    if (there[1] && p.out_type == kBf16 && p.width % 2 == 0) {
-                        reinterpret_cast<uint32_t *>(p.dweight)[at / 2] = to_bf16x2(x.x, x.y);
-                        continue;
-                    }
-                    if (there[0])
-                        store_param(p.dweight, p.out_type, at, x.x);
-                    if (there[1])
-                        store_param(p.dweight, p.out_type, at + 1, x.y);
-                }
-            }
-        }
+        if (ok)
+            store_tile(p, tmem, reinterpret_cast<float *>(ring) + warp * 32 * kStageRow, o0, tile_k0, part);
         tensor_fence_before();
+        if (!ok && lane == 0)
+            st_release_sys_u32(p.fault, kPipelineTimeout);
     }
     __syncthreads();
+    cluster_sync();  // neither block goes while the other may reach into it
     if (warp == kMmaWarp) {
         tensor_fence_after();
         tmem_free(tmem, kTmemColumns);
         if (lane == 0 && s.failed != 0)
             st_release_sys_u32(p.fault, kPipelineTimeout);
     }
-    if (warp < kDecodeWarps && !ok && lane == 0)
-        st_release_sys_u32(p.fault, kPipelineTimeout);
 }
 
 // Adds the parts of the rows in order, and folds the norm in.
@@ -477,21 +508,22 @@ void plan_weight_grad(WeightGradParams &p, int num_sms) {
     const int64_t want = int64_t(num_sms) * 4 * 32 / p.out + 1, most = (p.rows + 31) / 32;
     p.sum_rows = uint32_t(std::min(want, most));
     p.planes = p.type == kBf16 ? 1 : p.type == kFp16 ? 2 : 3;
-    p.halves = p.out > 128 ? 2 : 1;
-    p.tiles_o = (p.out + p.halves * 128 - 1) / (p.halves * 128);
-    const int64_t steps = (p.rows + kSteps - 1) / kSteps * p.planes;
-    // Cycles of one block: a stage is bound by its MMAs (128 x 16 x n takes n / 2)
-    // or its decoding (about 20 values a cycle); the epilogue moves ~12 values a
-    // cycle.  Splitting the rows costs a pass over the parts at ~3.5 KB a cycle.
+    p.halves = p.out > 256 ? 2 : 1;
+    p.tiles_o = (p.out + p.halves * 256 - 1) / (p.halves * 256);
+    const int64_t steps = (p.rows + kSteps - 1) / kSteps * p.planes, pairs = num_sms / 2;
+    // Cycles of one pair: a stage is bound by its MMAs (256 x 16 x n takes n / 2)
+    // or by shared memory (128 bytes a cycle: dy in and out, codes in and out,
+    // operands in, and out for each half); the epilogue moves ~12 values a cycle
+    // and block.  Splitting the rows costs a pass over the parts at ~3.5 KB a cycle.
     double best = 1e300;
-    for (uint32_t tile = 16; tile <= 256; tile += 16) {
+    for (uint32_t tile = 32; tile <= 256; tile += 32) {
         const uint32_t tiles_k = (p.width + tile - 1) / tile;
         const int64_t tiles = int64_t(p.tiles_o) * tiles_k;
         for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 64); parts = parts < 8 ? parts + 1 : parts * 2) {
             const int64_t part_steps = (steps + parts - 1) / parts, used = (steps + part_steps - 1) / part_steps;
-            const double waves = double((tiles * used + num_sms - 1) / num_sms);
-            const double stage = std::max(2.0 * p.halves * tile, 64.0 * tile / 20 + 150);
-            const double block = 3000 + part_steps * stage + p.halves * 128.0 * tile / 12;
+            const double waves = double((tiles * used + pairs - 1) / pairs);
+            const double stage = std::max({2.0 * p.halves * tile, 256.0 * p.halves + (1 + p.halves / 2.) * tile, 400.});
+            const double block = 5000 + part_steps * stage + p.halves * 128.0 * tile / 12;
             const double join = used > 1 ? 3000 + 8.0 * used * p.out * p.width / 3500 : 0;
             const double cost = waves * block + join;
             if (cost < best * 0.999) {
@@ -521,7 +553,7 @@ cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
     cudaError_t rc = cudaFuncSetAttribute(weight_grad_tensor, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess)
         return rc;
-    weight_grad_tensor<<<p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(p, dy_map, code_map);
+    weight_grad_tensor<<<2 * p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(p, dy_map, code_map);
     if (p.parts > 1) {
         const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
         weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(p);
