@@ -85,7 +85,7 @@ struct WeightGradParams {
     const void *norm_weight, *norm_bias;  // nullptr: not folded
     void *dweight, *dbias;                // dbias nullptr: not wanted
     float *dy_sums;                       // [out] fp32 column sums of dy; nullptr: not needed
-    float *sum_parts;                     // [sum_rows][out]
+    float *sum_parts;                     // [sum_rows][out], what dy_sums adds up
     void *dy_planes;                      // fp16, fp32: [planes][rows][plane_stride] bf16
     float *dw_parts;                      // [parts][out][width], parts > 1
     uint32_t *fault;                      // host-mapped: set when a wait ran out
@@ -94,6 +94,7 @@ struct WeightGradParams {
     // The plan (plan_weight_grad): dy as `planes` bf16 terms; pairs of blocks for
     // `halves` x 256 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64.
     uint32_t planes, halves, tile_k, tiles_k, tiles_o, parts, part_steps;
+    uint32_t boxes;  // results leave by tiled stores
 };
 
 cudaError_t launch_norm_forward(const NormForwardParams &p, int num_sms, cudaStream_t stream);

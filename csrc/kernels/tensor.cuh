@@ -19,6 +19,19 @@ __device__ __forceinline__ void tensor_load_3d(void *dst_smem, const CUtensorMap
                  : "memory");
 }
 
+// Tiled copy of one box to (x, y, z); what lies outside the tensor is not
+// written.  A bulk group of the calling thread.
+__device__ __forceinline__ void tensor_store_3d(const CUtensorMap *map, int x, int y, int z, const void *src_smem) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(smem_addr(src_smem))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's groups still read shared memory.
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }

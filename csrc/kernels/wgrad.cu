@@ -25,37 +25,43 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------- column sums of dy
-// Sums over one part of the rows: a block takes 32 columns.
-template <uint32_t TYPE>
+// Sums over one part of the rows: a lane takes W adjacent columns (one vector
+// of 16-byte rows, or one column), the block's warps every eighth row.  The
+// product's kernel adds the parts up.
+template <uint32_t TYPE, int W>
 __global__ void __launch_bounds__(kThreads) dy_sums_part(const __grid_constant__ WeightGradParams p) {
-    __shared__ float s_sum[kThreads / 32][32];
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, o = blockIdx.x * 32 + lane;
+    __shared__ float s_sum[kThreads / 32][32 * W];
+    using T = typename Element<TYPE>::T;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, o = blockIdx.x * 32 * W + lane * W;
     const int64_t share = (p.rows + p.sum_rows - 1) / p.sum_rows;
     const int64_t first = int64_t(blockIdx.y) * share, last = min(first + share, p.rows);
-    float sum = 0.f;
+    float sum[W] = {};
     if (o < p.out)
-        for (int64_t r = first + warp; r < last; r += kThreads / 32)
-            sum += Element<TYPE>::get(static_cast<const typename Element<TYPE>::T *>(p.dy)[r * p.dy_stride + o]);
-    s_sum[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && o < p.out) {
+#pragma unroll 8
+        for (int64_t r = first + warp; r < last; r += kThreads / 32) {
+            const T *dy = static_cast<const T *>(p.dy) + r * p.dy_stride + o;
+            if constexpr (W == 1) {
+                sum[0] += Element<TYPE>::get(*dy);
+            } else {
+                T v[W];
+                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(dy));
 #pragma unroll
-        for (int w = 1; w < kThreads / 32; ++w)
-            sum += s_sum[w][lane];
-        p.sum_parts[int64_t(blockIdx.y) * p.out + o] = sum;
+                for (int e = 0; e < W; ++e)
+                    sum[e] += Element<TYPE>::get(v[e]);
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+        s_sum[warp][lane * W + e] = sum[e];
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < 32 * W; c += kThreads) {
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w)
+            total += s_sum[w][c];
+        if (blockIdx.x * 32 * W + c < p.out)
+            p.sum_parts[int64_t(blockIdx.y) * p.out + blockIdx.x * 32 * W + c] = total;
     }
-}
-
-__global__ void __launch_bounds__(kThreads) dy_sums_join(const __grid_constant__ WeightGradParams p) {
-    const uint32_t o = blockIdx.x * kThreads + threadIdx.x;
-    if (o >= p.out)
-        return;
-    float sum = 0.f;
-    for (uint32_t part = 0; part < p.sum_rows; ++part)
-        sum += p.sum_parts[int64_t(part) * p.out + o];
-    p.dy_sums[o] = sum;
-    if (p.dbias != nullptr)
-        store_param(p.dbias, p.out_type, o, sum);
 }
 
 // ---------------------------------------------------------------- dy as bf16 terms
@@ -89,10 +95,11 @@ constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
 constexpr uint32_t kDyBytes = 4 * kDyChunk, kCodeBytes = 2 * kCodeChunk, kOperandBytes = 2 * kDyChunk;
 constexpr uint32_t kRingBytes = kLoadStages * (kDyBytes + kCodeBytes) + kOperandStages * kOperandBytes;
 constexpr uint32_t kSharedBytes = kRingBytes + 1024;  // + alignment of the swizzled tiles
-constexpr int kDecodeWarps = 8, kLoadWarp = 8, kScaleWarp = 9, kMmaWarp = 10, kTensorThreads = 11 * 32;
+constexpr int kDecodeWarps = 8, kLoadWarp = 8, kScaleWarp = 9, kMmaWarp = 10, kSumWarp = 11, kTensorThreads = 12 * 32;
 constexpr uint32_t kBlocks = 2;              // 128-column blocks that a block's share touches at most
 constexpr uint32_t kTmemColumns = 512;
-constexpr uint32_t kStageRow = 68;           // floats per row of an epilogue tile: 16-byte stores meet all banks
+constexpr uint32_t kBoxBytes = 32 * 128;     // an epilogue box: 32 rows x 32 columns
+constexpr int kBoxes = 3;                    // of each warp
 constexpr uint64_t kWaitNs = 2000000000ull;  // far above any legal wait
 
 // How a row's 128-column block is decoded.  Four codes s eeee mmm become four
@@ -141,6 +148,8 @@ struct Shared {
     uint32_t tmem;
     uint32_t failed;
     Decoder decoders[kLoadStages][kBlocks][kSteps];
+    float row_sums[2 * 128];                   // of dy, for this block's outputs
+    alignas(16) float weight[256], bias[256];  // the folded norm's, for the pair's columns
 };
 
 __device__ __forceinline__ Vec16 load_shared16(uint32_t at) {
@@ -157,76 +166,91 @@ __device__ __forceinline__ void store_shared16(uint32_t at, const Vec16 &v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// A block's accumulators to memory: a warp turns 32 rows x 64 columns at a time
-// by way of its part `tile` of the ring, which is free by then (TMEM gives a
-// lane a row; rows are to be stored whole).
-__device__ __forceinline__ void store_tile(const WeightGradParams &p, uint32_t tmem, float *tile, uint32_t o0, uint32_t k0,
-                                           uint32_t part) {
+// A block's accumulators to memory, folding the norm in where no parts are to be
+// joined first.  A warp takes 32 rows x 32 columns at a time (TMEM gives a lane
+// a row) by way of boxes in its part of the ring, which is free by then: tiled
+// stores where rows are on 16-byte boundaries, else row by row.
+template <uint32_t TYPE>
+__device__ __forceinline__ void store_tile(const WeightGradParams &p, const CUtensorMap *map, const Shared &s, uint32_t tmem,
+                                           uint8_t *boxes, uint32_t o0, uint32_t k0, uint32_t part) {
+    constexpr uint32_t kSize = element_bytes(TYPE), kRow = 32 * kSize;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, columns = min(p.tile_k, p.width - k0);
     const uint32_t half = p.halves == 2 ? warp / 4 : 0, row0 = warp % 4 * 32;
     const uint32_t o_first = o0 + half * 256 + row0;
     if (o_first >= p.out)
         return;
-    const uint32_t o_rows = min(32u, p.out - o_first);
-    const bool direct = p.parts == 1, weighted = direct && p.norm_weight != nullptr, shifted = direct && p.norm_bias != nullptr;
-    const float row_sum = shifted && lane < o_rows ? p.dy_sums[o_first + lane] : 0.f;
-    const uint32_t out_bytes = direct ? element_bytes(p.out_type) : 4;
-    uint8_t *out = direct ? static_cast<uint8_t *>(p.dweight)
-                          : reinterpret_cast<uint8_t *>(p.dw_parts + int64_t(part) * p.out * p.width);
-    const uint32_t out_type = direct ? p.out_type : uint32_t(kFp32);
-    // Two columns of a lane in one store: both rows and pairs start on its boundary.
-    const bool pairs = p.width % 2 == 0;
-    for (uint32_t c0 = p.halves == 2 ? 0 : warp / 4 * 64; c0 < columns; c0 += p.halves == 2 ? 64 : 128) {
-        uint32_t v[2][32];
-        const uint32_t address = tmem + (row0 << 16) + half * 256 + c0;
-        tmem_load32(address, v[0]);
-        tmem_load32(address + 32, v[1]);
-        const uint32_t c = c0 + lane * 2, k = k0 + c;
-        const bool there0 = c < columns, there1 = c + 1 < columns;
-        float w0 = 1.f, w1 = 1.f, b0 = 0.f, b1 = 0.f;
+    const bool weighted = p.parts == 1 && p.norm_weight != nullptr, shifted = p.parts == 1 && p.norm_bias != nullptr;
+    const float row_sum = shifted ? s.row_sums[half * 128 + row0 + lane] : 0.f;
+    int box = 0;
+    for (uint32_t c0 = p.halves == 2 ? 0 : warp / 4 * 32; c0 < columns; c0 += p.halves == 2 ? 32 : 64) {
+        uint32_t v[32];
+        tmem_load32(tmem + (row0 << 16) + half * 256 + c0, v);
+        if (lane == 0)
+            bulk_wait_read<kBoxes - 1>();  // this box has been stored
+        __syncwarp();
+        tmem_wait_loads();
+        uint8_t *at = boxes + box * kBoxBytes;
+        float x[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c)  // accumulators are in the decoders' order: columns 0, 2, 1, 3
+            x[c] = __uint_as_float(v[c % 4 == 1 ? c + 1 : c % 4 == 2 ? c - 1 : c]);
         if (weighted) {
-            w0 = there0 ? load_param(p.norm_weight, p.param_type, k) : 0.f;
-            w1 = there1 ? load_param(p.norm_weight, p.param_type, k + 1) : 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float4 w = *reinterpret_cast<const float4 *>(s.weight + c0 + q * 4);
+                x[q * 4] *= w.x, x[q * 4 + 1] *= w.y, x[q * 4 + 2] *= w.z, x[q * 4 + 3] *= w.w;
+            }
         }
         if (shifted) {
-            b0 = there0 ? load_param(p.norm_bias, p.param_type, k) : 0.f;
-            b1 = there1 ? load_param(p.norm_bias, p.param_type, k + 1) : 0.f;
-        }
-        tmem_wait_loads();
-        __syncwarp();  // the tile's last rows have been read
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const uint32_t *f = &v[q / 8][q % 8 * 4];  // in the decoders' order: columns 0, 2, 1, 3
-            *reinterpret_cast<uint4 *>(tile + lane * kStageRow + q * 4) = make_uint4(f[0], f[2], f[1], f[3]);
+            for (int q = 0; q < 8; ++q) {
+                const float4 b = *reinterpret_cast<const float4 *>(s.bias + c0 + q * 4);
+                x[q * 4] += b.x * row_sum, x[q * 4 + 1] += b.y * row_sum;
+                x[q * 4 + 2] += b.z * row_sum, x[q * 4 + 3] += b.w * row_sum;
+            }
         }
-        __syncwarp();
-        uint8_t *at = out + (int64_t(o_first) * p.width + k) * out_bytes;
-        const int64_t row_bytes = int64_t(p.width) * out_bytes;
+        // Rows of 64 or 128 bytes with the stores' swizzle of that width.
+#pragma unroll
+        for (uint32_t q = 0; q < kRow / 16; ++q) {
+            uint4 w;
+            if constexpr (TYPE == kFp32)
+                w = make_uint4(__float_as_uint(x[q * 4]), __float_as_uint(x[q * 4 + 1]), __float_as_uint(x[q * 4 + 2]),
+                               __float_as_uint(x[q * 4 + 3]));
+            else if constexpr (TYPE == kBf16)
+                w = make_uint4(to_bf16x2(x[q * 8], x[q * 8 + 1]), to_bf16x2(x[q * 8 + 2], x[q * 8 + 3]),
+                               to_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), to_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            else
+                w = make_uint4(to_fp16x2(x[q * 8], x[q * 8 + 1]), to_fp16x2(x[q * 8 + 2], x[q * 8 + 3]),
+                               to_fp16x2(x[q * 8 + 4], x[q * 8 + 5]), to_fp16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            const uint32_t swizzled = TYPE == kFp32 ? q ^ (lane & 7) : q ^ (lane >> 1 & 3);
+            *reinterpret_cast<uint4 *>(at + lane * kRow + swizzled * 16) = w;
+        }
+        if (p.boxes) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                tensor_store_3d(map, int(k0 + c0), int(o_first), int(part), at);
+                bulk_commit();
+            }
+            box = box + 1 == kBoxes ? 0 : box + 1;
+        } else {
+            __syncwarp();
+            using T = typename Element<TYPE>::T;
+            T *out = p.parts == 1 ? static_cast<T *>(p.dweight)
+                                  : reinterpret_cast<T *>(p.dw_parts + int64_t(part) * p.out * p.width);
+            const uint32_t o_rows = min(32u, p.out - o_first), chunk = lane * kSize / 16;
+            if (c0 + lane < columns)
 #pragma unroll 8
-        for (uint32_t r = 0; r < o_rows; ++r, at += row_bytes) {
-            float2 x = *reinterpret_cast<const float2 *>(tile + r * kStageRow + lane * 2);
-            if (weighted) {
-                x.x *= w0;
-                x.y *= w1;
-            }
-            if (shifted) {
-                const float sum = __shfl_sync(0xFFFFFFFFu, row_sum, r);
-                x.x += b0 * sum;
-                x.y += b1 * sum;
-            }
-            if (pairs && there1) {
-                if (out_type == kFp32)
-                    *reinterpret_cast<float2 *>(at) = x;
-                else
-                    *reinterpret_cast<uint32_t *>(at) = out_type == kBf16 ? to_bf16x2(x.x, x.y) : to_fp16x2(x.x, x.y);
-            } else {
-                if (there0)
-                    store_param(at, out_type, 0, x.x);
-                if (there1)
-                    store_param(at, out_type, 1, x.y);
-            }
+                for (uint32_t r = 0; r < o_rows; ++r) {
+                    const uint32_t swizzled = TYPE == kFp32 ? chunk ^ (r & 7) : chunk ^ (r >> 1 & 3);
+                    out[int64_t(o_first + r) * p.width + k0 + c0 + lane] =
+                        *reinterpret_cast<const T *>(at + r * kRow + swizzled * 16 + lane * kSize % 16);
+                }
+            __syncwarp();
         }
     }
+    if (lane == 0)
+        bulk_wait_read<0>();
 }
 
 // A pair of blocks: halves x 256 outputs by tile_k columns over one part of the
@@ -239,10 +263,11 @@ __device__ __forceinline__ void store_tile(const WeightGradParams &p, uint32_t t
 // Warp 8 copies tiles of dy and codes into a ring of four stages; warps 0-7
 // decode a stage's codes into one of three operand buffers, by the factors
 // that warp 9 makes of its scales; the leader's warp 10 issues the MMAs of a
-// stage for both halves.  Accumulators fill TMEM (2 x 256 columns).
+// stage for both halves; warp 11 adds up the column sums of dy meanwhile.
+// Accumulators fill TMEM (2 x 256 columns).
 __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     weight_grad_tensor(const __grid_constant__ WeightGradParams p, const __grid_constant__ CUtensorMap dy_map,
-                       const __grid_constant__ CUtensorMap code_map) {
+                       const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap out_map) {
     extern __shared__ uint8_t s_raw[];
     __shared__ Shared s;
     uint8_t *ring = s_raw + ((1024u - (smem_addr(s_raw) & 1023u)) & 1023u);
@@ -374,6 +399,40 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
                     mbar_arrive(&s.loaded[at]);
                 load(i + kAhead, next[a]);
             }
+    } else if (warp == kSumWarp) {
+        const bool weighted = p.parts == 1 && p.norm_weight != nullptr, shifted = p.parts == 1 && p.norm_bias != nullptr;
+        for (uint32_t c = lane; c < p.tile_k; c += 32) {
+            const bool there = tile_k0 + c < p.width;
+            s.weight[c] = weighted && there ? load_param(p.norm_weight, p.param_type, tile_k0 + c) : 0.f;
+            s.bias[c] = shifted && there ? load_param(p.norm_bias, p.param_type, tile_k0 + c) : 0.f;
+        }
+        const bool told = tile_k0 == 0 && part == 0;  // to the join and the bias
+        if (p.dy_sums != nullptr && (shifted || told)) {
+            // A lane's eight outputs together: their loads are in flight at once.
+            float sum[8] = {};
+            uint32_t o[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                o[j] = o0 + j / 4 * 256 + j % 4 * 32 + lane;
+                if (j / 4 >= p.halves)
+                    o[j] = p.out;
+            }
+#pragma unroll 4
+            for (uint32_t r = 0; r < p.sum_rows; ++r)
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j)
+                    if (o[j] < p.out)
+                        sum[j] += p.sum_parts[int64_t(r) * p.out + o[j]];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                s.row_sums[j * 32 + lane] = sum[j];
+                if (told && o[j] < p.out) {
+                    p.dy_sums[o[j]] = sum[j];
+                    if (p.dbias != nullptr)
+                        store_param(p.dbias, p.out_type, o[j], sum[j]);
+                }
+            }
+        }
     } else {
         // A warp takes 32 rows and every fourth 16-byte unit of them: eight lanes
         // of one shared-memory phase are eight rows of one unit, which both
@@ -446,8 +505,16 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
         ok = mbar_wait_often(&s.done, 0, kWaitNs);
         ok = __all_sync(0xFFFFFFFFu, ok) && s.failed == 0;
         tensor_fence_after();
-        if (ok)
-            store_tile(p, tmem, reinterpret_cast<float *>(ring) + warp * 32 * kStageRow, o0, tile_k0, part);
+        if (ok) {
+            uint8_t *boxes = ring + warp * (kBoxes * kBoxBytes);
+            const uint32_t type = p.parts == 1 ? p.out_type : uint32_t(kFp32);
+            if (type == kBf16)
+                store_tile<kBf16>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+            else if (type == kFp16)
+                store_tile<kFp16>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+            else
+                store_tile<kFp32>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+        }
         tensor_fence_before();
         if (!ok && lane == 0)
             st_release_sys_u32(p.fault, kPipelineTimeout);
@@ -479,12 +546,12 @@ __global__ void __launch_bounds__(kThreads) weight_grad_join(const __grid_consta
     }
 }
 
-// [planes][rows][columns] with boxes of 64 rows x 64 columns; what lies outside reads as zero.
-CUtensorMap tile_map(CUtensorMapDataType type, const void *base, uint64_t columns, uint64_t rows,
-                     uint64_t planes, uint64_t row_bytes, CUtensorMapSwizzle swizzle) {
+// [planes][rows][columns] in boxes; what lies outside reads as zero.
+CUtensorMap tile_map(CUtensorMapDataType type, const void *base, uint64_t columns, uint64_t rows, uint64_t planes,
+                     uint64_t row_bytes, uint32_t box_columns, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
     CUtensorMap map;
     const cuuint64_t dims[3] = {columns, rows, planes}, strides[2] = {row_bytes, row_bytes * rows};
-    const cuuint32_t box[3] = {64, kSteps, 1}, steps[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {box_columns, box_rows, 1}, steps[3] = {1, 1, 1};
     check_cu(driver().TensorMapEncodeTiled(&map, type, 3, const_cast<void *>(base), dims, strides, box, steps,
                                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
@@ -493,9 +560,13 @@ CUtensorMap tile_map(CUtensorMapDataType type, const void *base, uint64_t column
 }
 
 template <uint32_t TYPE> void dy_passes(const WeightGradParams &p, cudaStream_t stream) {
+    constexpr int kVector = 16 / element_bytes(TYPE);
     if (p.dy_sums != nullptr) {
-        dy_sums_part<TYPE><<<dim3((p.out + 31) / 32, p.sum_rows), kThreads, 0, stream>>>(p);
-        dy_sums_join<<<(p.out + kThreads - 1) / kThreads, kThreads, 0, stream>>>(p);
+        if (on_boundary(p.dy, 16) && p.dy_stride % kVector == 0 && p.out % kVector == 0)
+            dy_sums_part<TYPE, kVector>
+                <<<dim3((p.out + 32 * kVector - 1) / (32 * kVector), p.sum_rows), kThreads, 0, stream>>>(p);
+        else
+            dy_sums_part<TYPE, 1><<<dim3((p.out + 31) / 32, p.sum_rows), kThreads, 0, stream>>>(p);
     }
     if (p.planes > 1)
         split_dy<TYPE><<<uint32_t(std::min<int64_t>((p.rows * p.out + kThreads - 1) / kThreads, 148 * 16)), kThreads, 0,
@@ -505,8 +576,8 @@ template <uint32_t TYPE> void dy_passes(const WeightGradParams &p, cudaStream_t 
 } // namespace
 
 void plan_weight_grad(WeightGradParams &p, int num_sms) {
-    const int64_t want = int64_t(num_sms) * 4 * 32 / p.out + 1, most = (p.rows + 31) / 32;
-    p.sum_rows = uint32_t(std::min(want, most));
+    // Few parts for the product's sum warp to add up; 16 rows each at least.
+    p.sum_rows = uint32_t(std::min<int64_t>((p.rows + 15) / 16, 32));
     p.planes = p.type == kBf16 ? 1 : p.type == kFp16 ? 2 : 3;
     p.halves = p.out > 256 ? 2 : 1;
     p.tiles_o = (p.out + p.halves * 256 - 1) / (p.halves * 256);
@@ -547,13 +618,25 @@ cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
     const bool split = p.planes > 1;
     const CUtensorMap dy_map =
         tile_map(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, split ? p.dy_planes : p.dy, p.out, p.rows, p.planes,
-                 uint64_t(split ? p.plane_stride : p.dy_stride) * 2, CU_TENSOR_MAP_SWIZZLE_128B);
+                 uint64_t(split ? p.plane_stride : p.dy_stride) * 2, 64, kSteps, CU_TENSOR_MAP_SWIZZLE_128B);
     const CUtensorMap code_map = tile_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, p.codes, p.width, p.rows, 1,
-                                          uint64_t(p.codes_stride), CU_TENSOR_MAP_SWIZZLE_64B);
+                                          uint64_t(p.codes_stride), 64, kSteps, CU_TENSOR_MAP_SWIZZLE_64B);
+    const uint32_t type = p.parts == 1 ? p.out_type : uint32_t(kFp32);
+    WeightGradParams q = p;
+    q.boxes = p.width * element_bytes(type) % 16 == 0;
+    CUtensorMap out_map = code_map;  // not used without boxes
+    if (q.boxes)
+        out_map = tile_map(type == kBf16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                           : type == kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                           p.parts == 1 ? p.dweight : p.dw_parts, p.width, p.out, p.parts,
+                           uint64_t(p.width) * element_bytes(type), 32, 32,
+                           type == kFp32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     cudaError_t rc = cudaFuncSetAttribute(weight_grad_tensor, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess)
         return rc;
-    weight_grad_tensor<<<2 * p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(p, dy_map, code_map);
+    weight_grad_tensor<<<2 * p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(q, dy_map, code_map,
+                                                                                                     out_map);
     if (p.parts > 1) {
         const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
         weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(p);
