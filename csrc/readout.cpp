@@ -4,6 +4,7 @@
 // everything runs on the current stream of the inputs' device, and outputs and
 // workspaces come from torch's allocator, so calls can be captured into graphs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
@@ -83,13 +84,19 @@ int sm_count(int device) { return at::cuda::getDeviceProperties(device)->multiPr
 
 void *data(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
 
+// New tensors, past the dispatcher (half of a small call's time was spent in it).
+Tensor empty(at::IntArrayRef size, ScalarType dtype, const Tensor &like) {
+    return at::detail::empty_cuda(size, dtype, like.device(), std::nullopt);
+}
+
 // Code rows start on 16-byte boundaries, so every kernel can read them in vectors.
 Tensor empty_codes(const Tensor &like, int64_t rows, int64_t width) {
-    return at::empty({rows, (width + 15) / 16 * 16}, like.options().dtype(ScalarType::Float8_e4m3fn)).narrow(1, 0, width);
+    return at::detail::empty_strided_cuda({rows, width}, {(width + 15) / 16 * 16, 1}, ScalarType::Float8_e4m3fn,
+                                          like.device());
 }
 
 Tensor empty_scales(const Tensor &like, int64_t rows, int64_t width) {
-    return at::empty({rows, (width + kCheckpointBlock - 1) / kCheckpointBlock}, like.options().dtype(ScalarType::Float));
+    return empty({rows, (width + kCheckpointBlock - 1) / kCheckpointBlock}, ScalarType::Float, like);
 }
 
 // Rows that start on 16-byte boundaries, one after the other.
@@ -162,12 +169,12 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
     need_params(weight, bias, width, out);
     const int device = need_device(x, {&weight, &bias, &scales});
     c10::cuda::CUDAGuard guard(device);
-    const Tensor y = at::empty({rows, width}, x.options().dtype(out));
+    const Tensor y = empty({rows, width}, out, x);
     OptTensor codes, code_scales, mean, rstd;
     if (keep != kKeepNothing)
-        rstd = at::empty({rows}, x.options().dtype(ScalarType::Float));
+        rstd = empty({rows}, ScalarType::Float, x);
     if (keep == kKeepStats)
-        mean = at::empty({rows}, x.options().dtype(ScalarType::Float));
+        mean = empty({rows}, ScalarType::Float, x);
     if (keep == kKeepFp8) {
         codes = empty_codes(x, rows, width);
         code_scales = empty_scales(x, rows, width);
@@ -222,11 +229,11 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
     c10::cuda::CUDAGuard guard(device);
     OptTensor dx, dweight, dbias, partial;
     if (want_dx)
-        dx = at::empty({rows, width}, dy.options());
+        dx = empty({rows, width}, dy.scalar_type(), dy);
     const bool params = want_params && weight.has_value();
     if (params) {
-        dweight = at::empty({width}, weight->options());
-        dbias = at::empty({width}, weight->options());
+        dweight = empty({width}, weight->scalar_type(), dy);
+        dbias = empty({width}, weight->scalar_type(), dy);
     }
     if (rows == 0) {
         if (params) {
@@ -264,7 +271,7 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
     const int sms = sm_count(device);
     if (params) {
         p.parts = norm_backward_parts(p, sms);
-        partial = at::empty({2, int64_t(p.parts), width}, dy.options().dtype(ScalarType::Float));
+        partial = empty({2, int64_t(p.parts), width}, ScalarType::Float, dy);
         p.partial = static_cast<float *>(partial->data_ptr());
     }
     check_cuda(launch_norm_backward(p, sms, at::cuda::getCurrentCUDAStream(device).stream()),
@@ -302,7 +309,7 @@ Tensor restore_fp8(const Tensor &codes, const Tensor &scales, ScalarType dtype) 
     const int device = need_device(codes, {&scales_opt});
     c10::cuda::CUDAGuard guard(device);
     const int64_t rows = codes.size(0), width = codes.size(1);
-    const Tensor x = at::empty({rows, width}, codes.options().dtype(dtype));
+    const Tensor x = empty({rows, width}, dtype, codes);
     if (rows > 0) {
         RestoreFp8Params p{};
         p.codes = static_cast<const uint8_t *>(codes.data_ptr());
@@ -334,11 +341,10 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     const OptTensor codes_opt = codes, scales_opt = scales;
     const int device = need_device(dy, {&codes_opt, &scales_opt, &norm_weight, &norm_bias});
     c10::cuda::CUDAGuard guard(device);
-    const auto options = dy.options().dtype(result), floats = dy.options().dtype(ScalarType::Float);
-    const Tensor dweight = at::empty({out, width}, options);
+    const Tensor dweight = empty({out, width}, result, dy);
     OptTensor dbias, sums;
     if (want_bias)
-        dbias = at::empty({out}, options);
+        dbias = empty({out}, result, dy);
     if (rows == 0) {
         dweight.zero_();
         if (dbias)
@@ -349,7 +355,7 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     // Tiled copies want rows on 16-byte boundaries; others are copied first.
     Tensor rows_dy = dy, rows_codes = codes;
     if (dy.scalar_type() == ScalarType::BFloat16 && !on_16_bytes(dy, 2)) {
-        rows_dy = at::empty({rows, (out + 7) / 8 * 8}, dy.options()).narrow(1, 0, out);
+        rows_dy = at::detail::empty_strided_cuda({rows, out}, {(out + 7) / 8 * 8, 1}, dy.scalar_type(), dy.device());
         rows_dy.copy_(dy);
     }
     if (!on_16_bytes(codes, 1)) {
@@ -378,17 +384,17 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     plan_weight_grad(p, sm_count(device));
     OptTensor planes, dw_parts;
     if (want_bias || norm_bias) {
-        sums = at::empty({int64_t(p.sum_rows) + 1, out}, floats);
+        sums = empty({int64_t(p.sum_rows) + 1, out}, ScalarType::Float, dy);
         p.dy_sums = static_cast<float *>(sums->data_ptr());
         p.sum_parts = p.dy_sums + out;
     }
     if (p.planes > 1) {
         p.plane_stride = (out + 7) / 8 * 8;
-        planes = at::empty({int64_t(p.planes), rows, p.plane_stride}, dy.options().dtype(ScalarType::BFloat16));
+        planes = empty({int64_t(p.planes), rows, p.plane_stride}, ScalarType::BFloat16, dy);
         p.dy_planes = planes->data_ptr();
     }
     if (p.parts > 1) {
-        dw_parts = at::empty({int64_t(p.parts), out, width}, floats);
+        dw_parts = empty({int64_t(p.parts), out, width}, ScalarType::Float, dy);
         p.dw_parts = static_cast<float *>(dw_parts->data_ptr());
     }
     check_cuda(launch_weight_grad(p, at::cuda::getCurrentCUDAStream(device).stream()), "launch weight gradient");
