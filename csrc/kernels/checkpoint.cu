@@ -111,40 +111,48 @@ __global__ void __launch_bounds__(kThreads) save_chunks(const __grid_constant__ 
     }
 }
 
-// Any width, stride and alignment: a warp takes blocks of 128 columns.
+// Any width, stride and alignment: a warp takes blocks of 128 columns, a lane
+// four adjacent ones, whose codes leave in one store (rows of codes start on
+// 16-byte boundaries).
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) save_any(const __grid_constant__ SaveFp8Params p) {
     const uint32_t lane = threadIdx.x % 32;
     for (Pieces q(p.rows, p.width, kCheckpointBlock); q.at < q.total; q.next()) {
-        float v[kUnroll][4];
+        typename Element<TYPE>::T raw[kUnroll][4];
         int64_t row[kUnroll];
         uint32_t block[kUnroll];
         bool there[kUnroll];
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {
             there[j] = q.place(j, row[j], block[j]);
-            const auto *x = static_cast<const typename Element<TYPE>::T *>(p.x) + row[j] * p.x_stride;
+            const uint32_t c = block[j] * kCheckpointBlock + lane * 4;
+            const auto *x = static_cast<const typename Element<TYPE>::T *>(p.x) + min(row[j], p.rows - 1) * p.x_stride;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t c = block[j] * kCheckpointBlock + i * 32 + lane;
-                v[j][i] = there[j] && c < p.width ? Element<TYPE>::get(x[c]) : 0.f;
-            }
+            for (int i = 0; i < 4; ++i)  // all in flight: no branch guards a load
+                raw[j][i] = x[min(c + i, p.width - 1)];
         }
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                amax = fmaxf(amax, finite_abs(v[j][i]));
-            const BlockScale scale = block_scale(lanes_max(amax));
-            if (!there[j])
-                break;
+            const uint32_t c = block[j] * kCheckpointBlock + lane * 4;
+            float v[4], amax = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t c = block[j] * kCheckpointBlock + i * 32 + lane;
-                if (c < p.width)
-                    p.codes[row[j] * p.codes_stride + c] = to_e4m3(v[j][i] * scale.down);
+                v[i] = c + i < p.width ? Element<TYPE>::get(raw[j][i]) : 0.f;
+                amax = fmaxf(amax, finite_abs(v[i]));
             }
+            const BlockScale scale = block_scale(lanes_max(amax));
+            if (!there[j] || c >= p.width)
+                continue;
+            uint32_t codes = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                codes |= uint32_t(to_e4m3(v[i] * scale.down)) << (8 * i);
+            uint8_t *to = p.codes + row[j] * p.codes_stride + c;
+            if (c + 4 <= p.width)
+                *reinterpret_cast<uint32_t *>(to) = codes;
+            else
+                for (uint32_t i = 0; c + i < p.width; ++i)
+                    to[i] = uint8_t(codes >> (8 * i));
             if (lane == 0)
                 p.scales[row[j] * q.across + block[j]] = scale.up;
         }
@@ -221,12 +229,11 @@ __global__ void __launch_bounds__(kThreads) restore_any(const __grid_constant__ 
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {
             there[j] = q.place(j, row[j], block[j]);
-            scale[j] = there[j] ? __ldg(p.scales + row[j] * p.scale_row_stride + block[j] * p.scale_col_stride) : 0.f;
+            const int64_t r = min(row[j], p.rows - 1);
+            scale[j] = __ldg(p.scales + r * p.scale_row_stride + block[j] * p.scale_col_stride);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t c = block[j] * kCheckpointBlock + i * 32 + lane;
-                code[j][i] = there[j] && c < p.width ? p.codes[row[j] * p.codes_stride + c] : 0;
-            }
+            for (int i = 0; i < 4; ++i)  // all in flight: no branch guards a load
+                code[j][i] = p.codes[r * p.codes_stride + min(block[j] * kCheckpointBlock + i * 32 + lane, p.width - 1)];
         }
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) {

@@ -294,6 +294,83 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     }
 }
 
+// Rows of 16- and 32-bit values of any width and alignment up to 16 T E columns,
+// one read: as above with single values for chunks, so every access is one
+// element (64 or 128 bytes of a warp together).  E is a multiple of four: a
+// warp's columns are whole checkpoint blocks.
+template <uint32_t IN, uint32_t PARAM, int E, bool FP8>
+__global__ void __launch_bounds__(E == 8 ? 768 : 1024, E == 8 ? 2 : 1)
+    norm_forward_elements(const __grid_constant__ NormForwardParams p, bool warp_rows) {
+    using T = typename Element<IN>::T;
+    using W = typename Element<PARAM>::T;
+    __shared__ WideSums s_sum[2];
+    const RowShare share(warp_rows, E);
+    const uint32_t lane = threadIdx.x % 32, rows = uint32_t(p.rows), c0 = share.chunk;
+    const float inv = 1.f / float(p.width);
+    const uint32_t blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
+    const W *weight = static_cast<const W *>(p.weight), *bias = static_cast<const W *>(p.bias);
+    for (uint32_t r = share.row; r < rows; r += share.step) {
+        const T *row = static_cast<const T *>(p.x) + r * p.x_stride;
+        T *y = static_cast<T *>(p.y) + int64_t(r) * p.width + c0;
+        float x[E], a = 0.f, b = 0.f;
+        T raw[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)  // all in flight: no branch guards a load
+            raw[j] = row[min(c0 + j * 32, p.width - 1)];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            x[j] = c0 + j * 32 < p.width ? Element<IN>::get(raw[j]) : 0.f;
+            a += x[j];
+        }
+        const float mean = (warp_rows ? lanes_sum(a) : wide_sum2(a, 0.f, s_sum[0]).x) * inv;
+        a = 0.f;
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (c0 + j * 32 < p.width) {
+                x[j] -= mean;
+                a += x[j];
+                b += x[j] * x[j];
+            }
+        const float2 sums = warp_rows ? lanes_sum2(a, b) : wide_sum2(a, b, s_sum[1]);
+        const float shift = sums.x * inv;
+        const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
+        if (share.leader && p.keep != kKeepNothing) {
+            if (p.keep == kKeepStats)
+                p.mean[r] = mean + shift;
+            p.rstd[r] = rstd;
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const uint32_t c = c0 + j * 32;
+            x[j] = c < p.width ? (x[j] - shift) * rstd : 0.f;
+            if (c < p.width) {
+                float v = x[j];
+                if (weight != nullptr)
+                    v *= Element<PARAM>::get(weight[c]);
+                if (bias != nullptr)
+                    v += Element<PARAM>::get(bias[c]);
+                y[j * 32] = Element<IN>::put(v);
+            }
+        }
+        if constexpr (FP8) {
+            uint8_t *codes = p.codes + r * p.codes_stride + c0;
+#pragma unroll
+            for (int q = 0; q < E / 4; ++q) {
+                const float *h = x + q * 4;
+                const BlockScale unit =
+                    block_scale(lanes_max(largest3(largest3(0.f, h[0], h[1]), h[2], h[3])));
+                const uint32_t c = c0 - lane + q * kCheckpointBlock;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j * 32 + lane < p.width)
+                        codes[(q * 4 + j) * 32] = to_e4m3(h[j] * unit.down);
+                if (lane == 0 && c < p.width)
+                    p.code_scales[int64_t(r) * blocks + c / kCheckpointBlock] = unit.up;
+            }
+        }
+    }
+}
+
 // A normalised value of the backward pass.
 template <uint32_t X> __device__ __forceinline__ float kept_value(const NormBackwardParams &p, int64_t r, uint32_t c) {
     if (X == kE4m3)
@@ -565,6 +642,95 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
     }
 }
 
+// The same for rows of any width and alignment, by single elements.
+template <uint32_t X, uint32_t DY, uint32_t PARAM, int E, int T>
+__global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
+    using D = typename Element<DY>::T;
+    using K = typename Element<X>::T;
+    using W = typename Element<PARAM>::T;
+    __shared__ WideSums s_sum[2];
+    __shared__ float s_part[8][32 * E];
+    const RowShare share(warp_rows, E);
+    const uint32_t rows = uint32_t(p.rows), c0 = share.chunk;
+    const float inv = 1.f / float(p.width);
+    const uint32_t last = p.width - 1;
+    float dw[E] = {}, db[E] = {}, w[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        w[j] = p.weight == nullptr ? 1.f : Element<PARAM>::get(static_cast<const W *>(p.weight)[min(c0 + j * 32, last)]);
+    uint32_t turn = 0;
+    for (uint32_t r = share.row; r < rows; r += share.step, turn ^= 1) {
+        const D *dy = static_cast<const D *>(p.dy) + r * p.dy_stride;
+        const K *kept = X == kE4m3 ? reinterpret_cast<const K *>(p.codes) + r * p.codes_stride
+                                   : static_cast<const K *>(p.x) + r * p.x_stride;
+        D *dx = static_cast<D *>(p.dx) + int64_t(r) * p.width + c0;
+        const float rstd = __ldg(p.rstd + r), mean = X == kE4m3 ? 0.f : __ldg(p.mean + r);
+        D raw_g[E];
+        K raw_h[E];
+        float scale[E / 4];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {  // all in flight: no branch guards a load
+            const uint32_t c = min(c0 + j * 32, last);
+            raw_g[j] = dy[c];
+            raw_h[j] = kept[c];
+        }
+        if constexpr (X == kE4m3) {
+            const float *scales = p.code_scales + r * p.code_scales_stride;
+#pragma unroll
+            for (int q = 0; q < E / 4; ++q)
+                scale[q] = scales[min(c0 + q * kCheckpointBlock, last) / kCheckpointBlock * p.scale_col_stride];
+        }
+        float g[E], h[E], a = 0.f, b = 0.f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool there = c0 + j * 32 < p.width;
+            g[j] = there ? Element<DY>::get(raw_g[j]) : 0.f;
+            h[j] = X == kE4m3 ? Element<X>::get(raw_h[j]) * scale[j / 4] : (Element<X>::get(raw_h[j]) - mean) * rstd;
+            h[j] = there ? h[j] : 0.f;
+            dw[j] += g[j] * h[j];
+            db[j] += g[j];
+            g[j] *= w[j];
+            a += g[j];
+            b += g[j] * h[j];
+        }
+        const float2 sums = warp_rows ? lanes_sum2(a, b) : wide_sum2(a, b, s_sum[turn]);
+        if (p.dx != nullptr) {
+            const float c1 = sums.x * inv, c2 = sums.y * inv;
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (c0 + j * 32 < p.width)
+                    dx[j * 32] = Element<DY>::put(rstd * (g[j] - c1 - h[j] * c2));
+        }
+    }
+    if (p.dweight == nullptr)
+        return;
+    float *part[2] = {p.partial + int64_t(blockIdx.x) * p.width, p.partial + int64_t(p.parts + blockIdx.x) * p.width};
+    if (!warp_rows) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (const uint32_t c = c0 + j * 32; c < p.width) {
+                part[0][c] = dw[j];
+                part[1][c] = db[j];
+            }
+        return;
+    }
+    // Warp rows: the block's warps hold sums of the same columns.
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            s_part[threadIdx.x / 32][c0 + j * 32] = which == 0 ? dw[j] : db[j];
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < p.width; c += blockDim.x) {
+            float sum = 0.f;
+            for (uint32_t w = 0; w < blockDim.x / 32; ++w)
+                sum += s_part[w][c];
+            part[which][c] = sum;
+        }
+    }
+}
+
 uint32_t row_grid(int64_t rows, int num_sms) {
     return uint32_t(rows < int64_t(num_sms) * 8 ? rows : int64_t(num_sms) * 8);
 }
@@ -612,8 +778,29 @@ cudaError_t forward_rows(const NormForwardParams &p, int num_sms, cudaStream_t s
                                : forward_row<IN, OUT, PARAM, 4, false, 384>(p, num_sms, stream);
 }
 
+template <uint32_t IN, uint32_t PARAM, int E>
+void forward_elements(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    const bool warp_rows = p.width <= 32 * E;
+    const uint32_t threads = warp_rows ? 128 : (p.width + 32 * E - 1) / (32 * E) * 32;
+    const int64_t groups = warp_rows ? (p.rows + 3) / 4 : p.rows;
+    const uint32_t grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * (2048 / threads)));
+    if (p.keep == kKeepFp8)
+        norm_forward_elements<IN, PARAM, E, true><<<grid, threads, 0, stream>>>(p, warp_rows);
+    else
+        norm_forward_elements<IN, PARAM, E, false><<<grid, threads, 0, stream>>>(p, warp_rows);
+}
+
 template <uint32_t IN, uint32_t OUT>
 cudaError_t forward(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    if (IN != kE4m3 && !whole_chunks(p) && p.width <= 16 * 1024) {
+        constexpr uint32_t kIn = IN == kE4m3 ? OUT : IN;
+        const bool wide = p.width > 6144 || (p.width > 256 && p.width <= 512);  // 512: a warp holds a row
+        if (p.param_type == kFp32)
+            wide ? forward_elements<kIn, kFp32, 16>(p, num_sms, stream) : forward_elements<kIn, kFp32, 8>(p, num_sms, stream);
+        else
+            wide ? forward_elements<kIn, kIn, 16>(p, num_sms, stream) : forward_elements<kIn, kIn, 8>(p, num_sms, stream);
+        return cudaGetLastError();
+    }
     if (!whole_chunks(p)) {
         norm_forward_any<IN, OUT><<<row_grid(p.rows, num_sms), kRowThreads, 0, stream>>>(p);
         return cudaGetLastError();
@@ -624,36 +811,44 @@ cudaError_t forward(const NormForwardParams &p, int num_sms, cudaStream_t stream
     return rc == cudaSuccess ? cudaGetLastError() : rc;
 }
 
-// How norm_backward_row takes a call; threads == 0: it cannot, and the kernels
-// for any width, stride and alignment do.
+// How norm_backward_row takes a call, or norm_backward_elements (`elements` per
+// thread); threads == 0: neither can, and the kernels for any width do.
 struct BackwardPlan {
     uint32_t threads, grid, shared;
-    int vectors;
+    int vectors, elements;
     bool warp_rows;
 };
 
 BackwardPlan backward_plan(const NormBackwardParams &p, int num_sms) {
     BackwardPlan plan{};
     const bool fp8 = p.keep == kKeepFp8;
-    const uint32_t dy_bytes = element_bytes(p.dy_type), x_bytes = fp8 ? 1 : dy_bytes;
+    const uint32_t dy_bytes = element_bytes(p.dy_type), x_bytes = fp8 ? 1 : dy_bytes, chunks = p.width / 8;
     const void *x = fp8 ? static_cast<const void *>(p.codes) : p.x;
     const int64_t x_stride = fp8 ? p.codes_stride : p.x_stride;
-    if (p.width % 8 != 0 || !on_boundary(p.dy, 16) || p.dy_stride * dy_bytes % 16 != 0 || !on_boundary(x, 16) ||
-        x_stride * x_bytes % 16 != 0 || p.width * x_bytes % 16 != 0 || !on_boundary(p.weight, p.param_type == kFp32 ? 32 : 16))
-        return plan;
-    const uint32_t chunks = p.width / 8;
     plan.vectors = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
     plan.warp_rows = chunks <= 32u * plan.vectors;
-    const uint32_t threads = plan.warp_rows ? 256 : (chunks + 32 * plan.vectors - 1) / (32 * plan.vectors) * 32;
-    plan.shared = threads * plan.vectors * ring_depth(p.dy_type) * 8 * (dy_bytes + x_bytes);
+    plan.threads = plan.warp_rows ? 256 : (chunks + 32 * plan.vectors - 1) / (32 * plan.vectors) * 32;
+    plan.shared = plan.threads * plan.vectors * ring_depth(p.dy_type) * 8 * (dy_bytes + x_bytes);
     if (plan.warp_rows)
-        plan.shared = std::max(plan.shared, threads / 32 * p.width * 4);
-    if (threads > 512 || plan.shared > 200 * 1024)
-        return plan;
-    plan.threads = threads;
-    const int64_t groups = plan.warp_rows ? (p.rows + threads / 32 - 1) / (threads / 32) : p.rows;
-    const uint32_t registers = plan.vectors == 4 && threads <= 384 ? 168 : 128;
-    plan.grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident(threads, registers, plan.shared)));
+        plan.shared = std::max(plan.shared, plan.threads / 32 * p.width * 4);
+    uint32_t registers = plan.vectors == 4 && plan.threads <= 384 ? 168 : 128;
+    const bool boundaries = p.width % 8 == 0 && on_boundary(p.dy, 16) && p.dy_stride * dy_bytes % 16 == 0 &&
+                            on_boundary(x, 16) && x_stride * x_bytes % 16 == 0 && p.width * x_bytes % 16 == 0 &&
+                            on_boundary(p.weight, p.param_type == kFp32 ? 32 : 16);
+    if (!boundaries || plan.threads > 512 || plan.shared > 200 * 1024) {
+        if (p.width > 12288)
+            return BackwardPlan{};
+        plan.elements = p.width > 4096 || (p.width > 256 && p.width <= 512) ? 16 : 8;  // 512: a warp holds a row
+        plan.warp_rows = p.width <= 32u * plan.elements;
+        plan.threads = plan.warp_rows ? 256 : (p.width + 32 * plan.elements - 1) / (32 * plan.elements) * 32;
+        plan.shared = 0;
+        registers = plan.elements == 8 ? 64 : plan.threads <= 512 ? 128 : 84;
+    }
+    const int64_t groups = plan.warp_rows ? (p.rows + plan.threads / 32 - 1) / (plan.threads / 32) : p.rows;
+    // Each block leaves a part of the column sums: at least four rows for each,
+    // or the parts would be as much to move as the rows.
+    const int64_t most = p.dweight == nullptr ? groups : std::max<int64_t>(num_sms, groups / 4);
+    plan.grid = uint32_t(std::min({groups, most, int64_t(num_sms) * resident(plan.threads, registers, plan.shared)}));
     return plan;
 }
 
@@ -670,6 +865,14 @@ cudaError_t backward_row(const NormBackwardParams &p, const BackwardPlan &plan, 
 
 template <uint32_t X, uint32_t DY, uint32_t PARAM>
 cudaError_t backward_rows(const NormBackwardParams &p, const BackwardPlan &plan, cudaStream_t stream) {
+    if (plan.elements == 8)
+        norm_backward_elements<X, DY, PARAM, 8, 512><<<plan.grid, plan.threads, 0, stream>>>(p, plan.warp_rows);
+    else if (plan.elements == 16 && plan.threads <= 512)
+        norm_backward_elements<X, DY, PARAM, 16, 512><<<plan.grid, plan.threads, 0, stream>>>(p, plan.warp_rows);
+    else if (plan.elements == 16)
+        norm_backward_elements<X, DY, PARAM, 16, 768><<<plan.grid, plan.threads, 0, stream>>>(p, plan.warp_rows);
+    if (plan.elements != 0)
+        return cudaSuccess;
     return plan.vectors == 1    ? backward_row<X, DY, PARAM, 1, 256>(p, plan, stream)
            : plan.vectors == 2  ? backward_row<X, DY, PARAM, 2, 256>(p, plan, stream)
            : plan.threads > 384 ? backward_row<X, DY, PARAM, 4, 512>(p, plan, stream)

@@ -175,6 +175,20 @@ __device__ __forceinline__ float block_sum(float a, WarpSums &shared) {
     return a;
 }
 
+// block_sum2 for up to 32 warps.
+struct WideSums {
+    float2 of[32];
+};
+__device__ __forceinline__ float2 wide_sum2(float a, float b, WideSums &shared) {
+    const uint32_t lane = threadIdx.x % 32;
+    const float2 own = lanes_sum2(a, b);
+    if (lane == 0)
+        shared.of[threadIdx.x / 32] = own;
+    __syncthreads();
+    const float2 v = lane < blockDim.x / 32 ? shared.of[lane] : make_float2(0.f, 0.f);
+    return lanes_sum2(v.x, v.y);
+}
+
 // Eight adjacent values as they lie in memory: 16 bytes of a 16-bit type, 32
 // of fp32, 8 of codes.  Rows are streamed past L1; parameters stay in it.
 template <uint32_t TYPE> struct Raw8 {
