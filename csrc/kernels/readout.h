@@ -77,7 +77,8 @@ struct RestoreFp8Params {
 
 // dweight[o][k] = sum over rows of dy[row][o] * X[row][k], X the rows of an
 // 8-bit checkpoint; with a norm folded in, X * norm_weight + norm_bias.
-// Code rows, and bf16 dy rows, start on 16-byte boundaries.
+// Code rows start on 16-byte boundaries, and so do those of a bf16 dy without
+// dy_planes.
 struct WeightGradParams {
     const void *dy;
     const uint8_t *codes;
@@ -86,7 +87,7 @@ struct WeightGradParams {
     void *dweight, *dbias;                // dbias nullptr: not wanted
     float *dy_sums;                       // [out] fp32 column sums of dy; nullptr: not needed
     float *sum_parts;                     // [sum_rows][out], what dy_sums adds up
-    void *dy_planes;                      // fp16, fp32: [planes][rows][plane_stride] bf16
+    void *dy_planes;                      // [planes][rows][plane_stride] bf16; nullptr: dy itself serves
     float *dw_parts;                      // [parts][out][width], parts > 1
     uint32_t *fault;                      // host-mapped: set when a wait ran out
     int64_t rows, dy_stride, codes_stride, scale_row_stride, scale_col_stride, plane_stride;

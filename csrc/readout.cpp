@@ -353,17 +353,13 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     }
     uint32_t *fault = healthy_word(device);
     // Tiled copies want rows on 16-byte boundaries; others are copied first.
-    Tensor rows_dy = dy, rows_codes = codes;
-    if (dy.scalar_type() == ScalarType::BFloat16 && !on_16_bytes(dy, 2)) {
-        rows_dy = at::detail::empty_strided_cuda({rows, out}, {(out + 7) / 8 * 8, 1}, dy.scalar_type(), dy.device());
-        rows_dy.copy_(dy);
-    }
+    Tensor rows_codes = codes;
     if (!on_16_bytes(codes, 1)) {
         rows_codes = empty_codes(codes, rows, width);
         rows_codes.copy_(codes);
     }
     WeightGradParams p{};
-    p.dy = rows_dy.data_ptr();
+    p.dy = dy.data_ptr();
     p.codes = static_cast<const uint8_t *>(rows_codes.data_ptr());
     p.scales = static_cast<const float *>(scales.data_ptr());
     p.norm_weight = data(norm_weight);
@@ -372,7 +368,7 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
     p.dbias = data(dbias);
     p.fault = fault;
     p.rows = rows;
-    p.dy_stride = rows_dy.stride(0);
+    p.dy_stride = dy.stride(0);
     p.codes_stride = rows_codes.stride(0);
     p.scale_row_stride = scales.stride(0);
     p.scale_col_stride = scales.stride(1);
@@ -388,7 +384,7 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
         p.dy_sums = static_cast<float *>(sums->data_ptr());
         p.sum_parts = p.dy_sums + out;
     }
-    if (p.planes > 1) {
+    if (p.planes > 1 || !on_16_bytes(dy, 2)) {
         p.plane_stride = (out + 7) / 8 * 8;
         planes = empty({int64_t(p.planes), rows, p.plane_stride}, ScalarType::BFloat16, dy);
         p.dy_planes = planes->data_ptr();
