@@ -298,40 +298,51 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
 // one read: as above with single values for chunks, so every access is one
 // element (64 or 128 bytes of a warp together).  E is a multiple of four: a
 // warp's columns are whole checkpoint blocks.
-template <uint32_t IN, uint32_t PARAM, int E, bool FP8>
-__global__ void __launch_bounds__(E == 8 ? 768 : 1024, E == 8 ? 2 : 1)
+template <uint32_t IN, uint32_t PARAM, int E, bool FP8, int T0>
+__global__ void __launch_bounds__(T0, 1024 / T0)
     norm_forward_elements(const __grid_constant__ NormForwardParams p, bool warp_rows) {
     using T = typename Element<IN>::T;
     using W = typename Element<PARAM>::T;
-    __shared__ WideSums s_sum[2];
+    __shared__ RowSums<T0> s_sum[2];
     const RowShare share(warp_rows, E);
+    s_sum[0].clear();
+    s_sum[1].clear();
+    __syncthreads();
     const uint32_t lane = threadIdx.x % 32, rows = uint32_t(p.rows), c0 = share.chunk;
     const float inv = 1.f / float(p.width);
     const uint32_t blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
     const W *weight = static_cast<const W *>(p.weight), *bias = static_cast<const W *>(p.bias);
+    const bool whole = c0 - lane + 32 * E <= p.width;  // this warp's columns all exist
     for (uint32_t r = share.row; r < rows; r += share.step) {
         const T *row = static_cast<const T *>(p.x) + r * p.x_stride;
         T *y = static_cast<T *>(p.y) + int64_t(r) * p.width + c0;
         float x[E], a = 0.f, b = 0.f;
         T raw[E];
+        // All in flight: no branch guards a single load.
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < E; ++j)  // all in flight: no branch guards a load
-            raw[j] = row[min(c0 + j * 32, p.width - 1)];
+            for (int j = 0; j < E; ++j)
+                raw[j] = row[c0 + j * 32];
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                raw[j] = row[min(c0 + j * 32, p.width - 1)];
+        }
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            x[j] = c0 + j * 32 < p.width ? Element<IN>::get(raw[j]) : 0.f;
+            x[j] = whole || c0 + j * 32 < p.width ? Element<IN>::get(raw[j]) : 0.f;
             a += x[j];
         }
-        const float mean = (warp_rows ? lanes_sum(a) : wide_sum2(a, 0.f, s_sum[0]).x) * inv;
+        const float mean = (warp_rows ? lanes_sum(a) : s_sum[0].sum(a)) * inv;
         a = 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j)
-            if (c0 + j * 32 < p.width) {
+            if (whole || c0 + j * 32 < p.width) {
                 x[j] -= mean;
                 a += x[j];
                 b += x[j] * x[j];
             }
-        const float2 sums = warp_rows ? lanes_sum2(a, b) : wide_sum2(a, b, s_sum[1]);
+        const float2 sums = warp_rows ? lanes_sum2(a, b) : s_sum[1].sum2(a, b);
         const float shift = sums.x * inv;
         const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
         if (share.leader && p.keep != kKeepNothing) {
@@ -339,18 +350,29 @@ __global__ void __launch_bounds__(E == 8 ? 768 : 1024, E == 8 ? 2 : 1)
                 p.mean[r] = mean + shift;
             p.rstd[r] = rstd;
         }
+        float v[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            const uint32_t c = c0 + j * 32;
-            x[j] = c < p.width ? (x[j] - shift) * rstd : 0.f;
-            if (c < p.width) {
-                float v = x[j];
-                if (weight != nullptr)
-                    v *= Element<PARAM>::get(weight[c]);
-                if (bias != nullptr)
-                    v += Element<PARAM>::get(bias[c]);
-                y[j * 32] = Element<IN>::put(v);
-            }
+            x[j] = whole || c0 + j * 32 < p.width ? (x[j] - shift) * rstd : 0.f;
+            v[j] = x[j];
+        }
+        if (weight != nullptr)
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                v[j] *= Element<PARAM>::get(__ldg(weight + (whole ? c0 + j * 32 : min(c0 + j * 32, p.width - 1))));
+        if (bias != nullptr)
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                v[j] += Element<PARAM>::get(__ldg(bias + (whole ? c0 + j * 32 : min(c0 + j * 32, p.width - 1))));
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                y[j * 32] = Element<IN>::put(v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (c0 + j * 32 < p.width)
+                    y[j * 32] = Element<IN>::put(v[j]);
         }
         if constexpr (FP8) {
             uint8_t *codes = p.codes + r * p.codes_stride + c0;
@@ -450,7 +472,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
     const float *partial = p.partial + int64_t(blockIdx.y) * p.parts * p.width + c;
     float sum = 0.f;
     if (c < p.width)
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t part = warp; part < p.parts; part += kJoinWarps)
             sum += __ldg(partial + int64_t(part) * p.width);
     s_sum[warp][lane] = sum;
@@ -648,9 +670,12 @@ __global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(cons
     using D = typename Element<DY>::T;
     using K = typename Element<X>::T;
     using W = typename Element<PARAM>::T;
-    __shared__ WideSums s_sum[2];
+    __shared__ RowSums<T> s_sum[2];
     __shared__ float s_part[8][32 * E];
     const RowShare share(warp_rows, E);
+    s_sum[0].clear();
+    s_sum[1].clear();
+    __syncthreads();
     const uint32_t rows = uint32_t(p.rows), c0 = share.chunk;
     const float inv = 1.f / float(p.width);
     const uint32_t last = p.width - 1;
@@ -693,7 +718,7 @@ __global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(cons
             a += g[j];
             b += g[j] * h[j];
         }
-        const float2 sums = warp_rows ? lanes_sum2(a, b) : wide_sum2(a, b, s_sum[turn]);
+        const float2 sums = warp_rows ? lanes_sum2(a, b) : s_sum[turn].sum2(a, b);
         if (p.dx != nullptr) {
             const float c1 = sums.x * inv, c2 = sums.y * inv;
 #pragma unroll
@@ -778,27 +803,35 @@ cudaError_t forward_rows(const NormForwardParams &p, int num_sms, cudaStream_t s
                                : forward_row<IN, OUT, PARAM, 4, false, 384>(p, num_sms, stream);
 }
 
-template <uint32_t IN, uint32_t PARAM, int E>
+template <uint32_t IN, uint32_t PARAM, int E, int T>
 void forward_elements(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
     const bool warp_rows = p.width <= 32 * E;
     const uint32_t threads = warp_rows ? 128 : (p.width + 32 * E - 1) / (32 * E) * 32;
     const int64_t groups = warp_rows ? (p.rows + 3) / 4 : p.rows;
-    const uint32_t grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * (2048 / threads)));
+    const uint32_t grid = uint32_t(std::min<int64_t>(groups, int64_t(num_sms) * resident(threads, 64, 0)));
     if (p.keep == kKeepFp8)
-        norm_forward_elements<IN, PARAM, E, true><<<grid, threads, 0, stream>>>(p, warp_rows);
+        norm_forward_elements<IN, PARAM, E, true, T><<<grid, threads, 0, stream>>>(p, warp_rows);
     else
-        norm_forward_elements<IN, PARAM, E, false><<<grid, threads, 0, stream>>>(p, warp_rows);
+        norm_forward_elements<IN, PARAM, E, false, T><<<grid, threads, 0, stream>>>(p, warp_rows);
+}
+
+template <uint32_t IN, uint32_t PARAM> void forward_elements(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
+    if (p.width <= 256)
+        forward_elements<IN, PARAM, 8, 512>(p, num_sms, stream);
+    else if (p.width <= 8192)
+        forward_elements<IN, PARAM, 16, 512>(p, num_sms, stream);
+    else
+        forward_elements<IN, PARAM, 16, 1024>(p, num_sms, stream);
 }
 
 template <uint32_t IN, uint32_t OUT>
 cudaError_t forward(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
     if (IN != kE4m3 && !whole_chunks(p) && p.width <= 16 * 1024) {
         constexpr uint32_t kIn = IN == kE4m3 ? OUT : IN;
-        const bool wide = p.width > 6144 || (p.width > 256 && p.width <= 512);  // 512: a warp holds a row
         if (p.param_type == kFp32)
-            wide ? forward_elements<kIn, kFp32, 16>(p, num_sms, stream) : forward_elements<kIn, kFp32, 8>(p, num_sms, stream);
+            forward_elements<kIn, kFp32>(p, num_sms, stream);
         else
-            wide ? forward_elements<kIn, kIn, 16>(p, num_sms, stream) : forward_elements<kIn, kIn, 8>(p, num_sms, stream);
+            forward_elements<kIn, kIn>(p, num_sms, stream);
         return cudaGetLastError();
     }
     if (!whole_chunks(p)) {
@@ -845,9 +878,9 @@ BackwardPlan backward_plan(const NormBackwardParams &p, int num_sms) {
         registers = plan.elements == 8 ? 64 : plan.threads <= 512 ? 128 : 84;
     }
     const int64_t groups = plan.warp_rows ? (p.rows + plan.threads / 32 - 1) / (plan.threads / 32) : p.rows;
-    // Each block leaves a part of the column sums: at least four rows for each,
-    // or the parts would be as much to move as the rows.
-    const int64_t most = p.dweight == nullptr ? groups : std::max<int64_t>(num_sms, groups / 4);
+    // Each block leaves a part of the column sums: eight rows for each where there
+    // are enough, or the parts would be as much to move and add up as the rows.
+    const int64_t most = p.dweight == nullptr ? groups : std::max<int64_t>(2 * num_sms, groups / 8);
     plan.grid = uint32_t(std::min({groups, most, int64_t(num_sms) * resident(plan.threads, registers, plan.shared)}));
     return plan;
 }

@@ -175,19 +175,28 @@ __device__ __forceinline__ float block_sum(float a, WarpSums &shared) {
     return a;
 }
 
-// block_sum2 for up to 32 warps.
+// The same for blocks of up to T threads, more than 16 warps by pairs in lanes.
+template <int T> struct RowSums : WarpSums {
+    __device__ __forceinline__ void clear() { clear_sums(*this); }
+    __device__ __forceinline__ float sum(float a) { return block_sum(a, *this); }
+    __device__ __forceinline__ float2 sum2(float a, float b) { return block_sum2(a, b, *this); }
+};
 struct WideSums {
     float2 of[32];
+    __device__ __forceinline__ void clear() {}
+    __device__ __forceinline__ float sum(float a) { return sum2(a, 0.f).x; }
+    __device__ __forceinline__ float2 sum2(float a, float b) {
+        const uint32_t lane = threadIdx.x % 32;
+        const float2 own = lanes_sum2(a, b);
+        if (lane == 0)
+            of[threadIdx.x / 32] = own;
+        __syncthreads();
+        const float2 v = lane < blockDim.x / 32 ? of[lane] : make_float2(0.f, 0.f);
+        return lanes_sum2(v.x, v.y);
+    }
 };
-__device__ __forceinline__ float2 wide_sum2(float a, float b, WideSums &shared) {
-    const uint32_t lane = threadIdx.x % 32;
-    const float2 own = lanes_sum2(a, b);
-    if (lane == 0)
-        shared.of[threadIdx.x / 32] = own;
-    __syncthreads();
-    const float2 v = lane < blockDim.x / 32 ? shared.of[lane] : make_float2(0.f, 0.f);
-    return lanes_sum2(v.x, v.y);
-}
+template <> struct RowSums<768> : WideSums {};
+template <> struct RowSums<1024> : WideSums {};
 
 // Eight adjacent values as they lie in memory: 16 bytes of a 16-bit type, 32
 // of fp32, 8 of codes.  Rows are streamed past L1; parameters stay in it.
