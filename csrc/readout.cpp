@@ -14,6 +14,7 @@
 #include <cstring>
 #include <mutex>
 #include <optional>
+#include <utility>
 
 #include "bindings.h"
 #include "driver.h"
@@ -106,29 +107,35 @@ bool on_16_bytes(const Tensor &t, int64_t size) {
 }
 
 // One host-mapped word per device that a kernel sets when one of its bounded
-// waits ran out (its results are then not to be used).  It is read before every
-// launch, without synchronising, and a set one refuses all further ones.
-uint32_t *healthy_word(int device) {
+// waits ran out (its results are then not to be used).
+uint32_t *fault_word(int device) {
     static std::array<std::atomic<uint32_t *>, 64> words{};
     static std::mutex mutex;
     check(device >= 0 && device < int(words.size()), "device index out of range");
     uint32_t *word = words[device].load(std::memory_order_acquire);
+    if (word != nullptr)
+        return word;
+    std::lock_guard<std::mutex> lock(mutex);
+    word = words[device].load(std::memory_order_relaxed);
     if (word == nullptr) {
-        std::lock_guard<std::mutex> lock(mutex);
-        word = words[device].load(std::memory_order_relaxed);
-        if (word == nullptr) {
-            // Allowed while a graph is captured: the allocation is no part of it.
-            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-            check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
-            void *fresh = nullptr;
-            const cudaError_t rc = cudaHostAlloc(&fresh, 64, cudaHostAllocMapped | cudaHostAllocPortable);
-            cudaThreadExchangeStreamCaptureMode(&mode);
-            check_cuda(rc, "allocate fault word");
-            std::memset(fresh, 0, 64);
-            word = static_cast<uint32_t *>(fresh);
-            words[device].store(word, std::memory_order_release);
-        }
+        // Allowed while a graph is captured: the allocation is no part of it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+        void *fresh = nullptr;
+        const cudaError_t rc = cudaHostAlloc(&fresh, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        check_cuda(rc, "allocate fault word");
+        std::memset(fresh, 0, 64);
+        word = static_cast<uint32_t *>(fresh);
+        words[device].store(word, std::memory_order_release);
     }
+    return word;
+}
+
+// The word, read before every launch without synchronising: a set one refuses
+// all further launches.
+uint32_t *healthy_word(int device) {
+    uint32_t *word = fault_word(device);
     check(*static_cast<const volatile uint32_t *>(word) == 0,
           "an earlier read-out kernel on this GPU gave up waiting for its own copies; its results are invalid");
     return word;
@@ -404,6 +411,10 @@ void bind_readout(py::module_ &m) {
           py::arg("scales"), py::arg("hidden"), py::arg("block"), py::arg("dtype"), py::arg("keep"));
     m.def("norm_backward", &norm_backward, py::arg("dy"), py::arg("kept"), py::arg("scales"), py::arg("mean"),
           py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"));
+    m.def(
+        "debug_readout_fault",
+        [](int device, uint32_t code) { return std::exchange(*static_cast<volatile uint32_t *>(fault_word(device)), code); },
+        py::arg("device"), py::arg("code"), "Replace a device's fault word (tests of how a given-up wait is reported).");
     m.def("save_fp8", &save_fp8, py::arg("x"));
     m.def("restore_fp8", &restore_fp8, py::arg("codes"), py::arg("scales"), py::arg("dtype"));
     m.def("fp8_weight_grad", &fp8_weight_grad, py::arg("dy"), py::arg("codes"), py::arg("scales"),

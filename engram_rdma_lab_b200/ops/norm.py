@@ -8,7 +8,9 @@ with one (``keep="fp8"``; the format of :mod:`.checkpoint`), half of bf16's byte
 the gradient needs, and the same checkpoint serves the projection behind the norm
 (:func:`~.projection.fp8_weight_grad`).
 
-Sums over rows and columns are held in fp32 and joined in a fixed order: equal inputs give equal bits on equal GPUs.
+Sums over rows and columns are held in fp32 and joined in a fixed order: equal inputs give equal bits on equal GPUs,
+and a row's ``y`` does not depend on the rows beside it.  Everything runs on the current stream and can be captured
+into CUDA graphs (capture the functional pair, not autograd's backward pass).
 """
 
 from __future__ import annotations
@@ -71,6 +73,11 @@ def _adjacent(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _no_code_gradient(x: torch.Tensor):
+    if x.dtype == torch.float8_e4m3fn and x.requires_grad:
+        raise ValueError("float8_e4m3fn rows get no gradient; layer_norm_backward gives their dequantised rows'")
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, scales, hidden, block, dtype, keep):
@@ -98,6 +105,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hid
     """
     if _keep_mode(keep) == 0:
         raise ValueError('keep must be "exact" or "fp8"')
+    _no_code_gradient(x)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps, scales, hidden, block, dtype, keep)
     return layer_norm_forward(x, weight, bias, eps, scales=scales, hidden=hidden, block=block, dtype=dtype)[0]

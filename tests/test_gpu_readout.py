@@ -458,6 +458,38 @@ def test_layer_norm_keeps_exact_rows_from_being_changed():
         y.sum().backward()
 
 
+# Widths at which another kernel, or another of its variants, takes the call: whole chunks in a warp (256, 512), in a
+# block (1024 and up), at the most (16384), past it; single elements in a warp (300), in a block (513, 8193), past it.
+@pytest.mark.parametrize("keep", ["exact", "fp8"])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("m,n", [(1200, 8), (700, 264), (700, 512), (300, 520), (500, 1024), (5, 1032), (300, 4096), (3, 12304),
+                                 (160, 16384), (4, 16400), (900, 300), (900, 511), (500, 513), (160, 8191), (160, 8193), (5, 12289),
+                                 (3, 16385), (2, 20001)])
+def test_norm_at_the_borders_of_its_variants(m, n, dtype, keep):
+    x = (randn(m + n, m, n) * 2 + randn(n, 1, n)).to(dtype)
+    dy = randn(m * 3 + n, m, n, dtype=dtype)
+    w, b = params(n, dtype)
+    want, h, _, rstd = norm_exact(x, w, b)
+    y, kept = layer_norm_forward(x, w, b, EPS, keep=keep)
+    close(y, want, y_tolerance(x, w, b, dtype), "y")
+    if keep == "fp8":
+        check_kept(kept, x, h, rstd)
+    for name, a, c in zip(("dx", "dweight", "dbias"), layer_norm_backward(dy, kept, w), backward_exact(dy, kept, w)):
+        close(a, *c, name)
+    # A row's bits do not depend on the rows beside it.
+    one, _ = layer_norm_forward(x[m - 1:], w, b, EPS)
+    assert torch.equal(one, y[m - 1:])
+
+
+def test_norm_of_many_looked_up_tokens():
+    codes, scales, x = lookup(3, 3000, 6, 256, 128)
+    w, b = params(1536, BF16)
+    y, kept = layer_norm_forward(codes, w, b, EPS, scales=scales, hidden=256, keep="fp8")
+    want, h, _, rstd = norm_exact(x, w, b)
+    close(y, want, y_tolerance(x, w, b, BF16), "y")
+    check_kept(kept, x, h, rstd)
+
+
 # ---------------------------------------------------------------- weight gradient
 def checkpoint(seed, m, n):
     return save_fp8(randn(seed, m, n) * torch.exp2(randn(seed + 1, 1, n)))
@@ -674,6 +706,52 @@ def test_calls_run_on_the_current_stream():
         got = step(*late, w, b)
     stream.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_a_wait_that_ran_out_refuses_what_follows():
+    """The word that a kernel sets when it gives up, set here by hand."""
+    from engram_rdma_lab_b200 import _native
+
+    C = _native.load()
+    x = randn(1, 4, 256, dtype=BF16)
+    codes, scales = save_fp8(x)
+    assert C.debug_readout_fault(0, 5) == 0
+    try:
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            layer_norm_forward(x)
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            fp8_weight_grad(x, codes, scales)
+    finally:
+        assert C.debug_readout_fault(0, 0) == 5
+    layer_norm_forward(x)
+
+
+def test_calls_from_several_threads():
+    """Two threads on streams of their own: nothing is shared between calls."""
+    import threading
+
+    m, n, out = 400, 1536, 200
+    w, b = params(n, BF16)
+    inputs = [[randn(s, m, n, dtype=BF16), randn(s + 1, m, n, dtype=BF16), randn(s + 2, m, out, dtype=BF16)] for s in (1, 5)]
+    want = [step(*values, w, b) for values in inputs]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = step(*inputs[k], w, b)
+        stream.synchronize()
+        if not all(torch.equal(a, c) for a, c in zip(got, want[k])):
+            failures.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
 
 
 def test_other_tensors_are_left_alone():

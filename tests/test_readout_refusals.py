@@ -63,6 +63,8 @@ def scales(m=4, n=2):
     (lambda: layer_norm_forward(rows(), torch.zeros(256), torch.zeros(256).bfloat16()), "bias must be"),
     (lambda: layer_norm_forward(rows()), "on a GPU"),
     (lambda: layer_norm(rows(), keep=None), "keep must be"),
+    (lambda: layer_norm(codes().requires_grad_(), scales=scales()), "get no gradient"),
+    (lambda: norm_linear(codes().requires_grad_(), None, None, rows(8), scales=scales()), "get no gradient"),
     (lambda: layer_norm_backward(rows(), KeptRows(rows(3), None, torch.zeros(3), torch.zeros(3))), "shape of the kept rows"),
     (lambda: layer_norm_backward(rows(dtype=torch.float16), KeptRows(rows(), None, torch.zeros(4), torch.zeros(4))), "rows' type"),
     (lambda: layer_norm_backward(rows(), KeptRows(rows(), None, None, torch.zeros(4))), "mean must be"),
