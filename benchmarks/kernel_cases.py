@@ -13,7 +13,12 @@ JSON line per case with the median CUDA-event time and the bytes moved:
 * ``push`` / ``hook``: the host route's serving code moving one request of
   ``--rows`` rows of this rank to itself, read zero-copy from the pinned host
   shard (or, with ``--mirror``, from the HBM mirror) by the push kernel
-  (``--blocks`` CTAs) or by a serving hook kernel.
+  (``--blocks`` CTAs) or by a serving hook kernel;
+* ``norm`` / ``norm_backward`` / ``save`` / ``restore`` / ``wgrad``: the
+  read-out operators on one fetched layer (FP8, 4096 tokens x 24 entries):
+  its layer norm kept in 8 bits, the backward pass from that checkpoint, bf16
+  activations of its shape to 8 bits and back, and the gradient of a
+  projection to ``--features`` behind the norm.
 
 Run: ``python benchmarks/kernel_cases.py --case gather [--launches 20]``.  Under
 ncu, capture one launch after the warm-up ones (``-k regex:<kernel> -s 3 -c 1``).
@@ -34,7 +39,7 @@ import torch.distributed as dist
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from engram_rdma_lab_b200 import EngramBuffer  # noqa: E402
+from engram_rdma_lab_b200 import EngramBuffer, ops  # noqa: E402
 from engram_rdma_lab_b200.models import make_indices, normal_bf16_shard, quantized_fp8_shard  # noqa: E402
 
 ENTRIES, HIDDEN, TOKENS, EPT = (524288, 524309), 256, 4096, 24
@@ -42,7 +47,9 @@ ENTRIES, HIDDEN, TOKENS, EPT = (524288, 524309), 256, 4096, 24
 
 def parse():
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    p.add_argument("--case", choices=["gather", "dedup", "push", "hook"], required=True)
+    p.add_argument("--case", required=True,
+                   choices=["gather", "dedup", "push", "hook", "norm", "norm_backward", "save", "restore", "wgrad"])
+    p.add_argument("--features", type=int, default=2048, help="outputs of the projection (wgrad)")
     p.add_argument("--launches", type=int, default=20)
     p.add_argument("--rows", type=int, default=98304, help="rows of the served request (push / hook)")
     p.add_argument("--blocks", default="8", help="push CTAs, comma-separated for a sweep")
@@ -82,6 +89,39 @@ def time_fetches(buf, distribution, launches):
     return statistics.median(samples[2:] if len(samples) > 4 else samples)
 
 
+def time_readout(buf, case, features, launches):
+    """(median us, bytes that one call has to move, floating-point operations)."""
+    indices = make_indices(0, 1, ENTRIES, TOKENS, EPT, device="cuda")
+    data, scales = (t.clone() for t in buf.fetch_all(indices)[0])
+    width = HIDDEN * EPT
+    g = torch.Generator(device="cuda").manual_seed(1)
+    weight = (1 + 0.1 * torch.randn(width, generator=g, device="cuda")).bfloat16()
+    bias = (0.1 * torch.randn(width, generator=g, device="cuda")).bfloat16()
+    dy = torch.randn(TOKENS, width, generator=g, device="cuda").bfloat16()
+    dz = torch.randn(TOKENS, features, generator=g, device="cuda").bfloat16()
+    _, kept = ops.layer_norm_forward(data, weight, bias, scales=scales, hidden=HIDDEN, keep="fp8")
+    cells = TOKENS * width
+    call, nbytes, flops = {
+        "norm": (lambda: ops.layer_norm_forward(data, weight, bias, scales=scales, hidden=HIDDEN, keep="fp8"), cells * 4, 0),
+        "norm_backward": (lambda: ops.layer_norm_backward(dy, kept, weight), cells * 5, 0),
+        "save": (lambda: ops.save_fp8(dy), cells * 3, 0),
+        "restore": (lambda: ops.restore_fp8(kept.rows, kept.scales), cells * 3, 0),
+        "wgrad": (lambda: ops.fp8_weight_grad(dz, kept.rows, kept.scales, weight, bias),
+                  cells + 2 * features * (TOKENS + width), 2 * cells * features),
+    }[case]
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")  # larger than L2
+    samples = []
+    for _ in range(launches):
+        flush.zero_()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        samples.append(a.elapsed_time(b) * 1e3)
+    return statistics.median(samples[2:] if len(samples) > 4 else samples), nbytes, flops
+
+
 def main():
     args = parse()
     torch.cuda.set_device(0)
@@ -102,6 +142,11 @@ def main():
                     algorithmic_bytes=nbytes, gbs=round(nbytes / (us * 1e-6) / 1e9, 1),
                     dedup_unique_ratio=mem["dedup_last_unique_ratio"])
         print(json.dumps(line), flush=True)
+    elif args.case not in ("push", "hook"):
+        buf = buffer(fp8=True, mirror=True)
+        us, nbytes, flops = time_readout(buf, args.case, args.features, args.launches)
+        print(json.dumps(dict(line, us=round(us, 2), bytes=nbytes, gbs=round(nbytes / us / 1e3, 1),
+                              tflops=round(flops / us / 1e6, 1))), flush=True)
     else:
         buf = buffer(fp8=False, mirror=args.mirror)
         line["source"] = "hbm_mirror" if args.mirror else "pinned_host_shard"

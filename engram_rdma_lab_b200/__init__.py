@@ -7,8 +7,10 @@ NVSwitch node, with the EngramBuffer API of yykzjh/engram-rdma-lab:
 * :class:`TorchEngramBuffer` - the same API on torch collectives (CPU/gloo
   oracle, NCCL ``all_to_all`` baseline);
 * :mod:`.routing` - route negotiation (``ENGRAM_EGM_ENABLE``);
-* :mod:`.models` - benchmark table sets, synthetic weights and index streams;
-* :mod:`.ops` - FP8 block quantisation helpers;
+* :mod:`.models` - benchmark table sets, synthetic weights and index streams, the
+  read-out module of a layer's rows;
+* :mod:`.ops` - FP8 block quantisation helpers, layer norm over looked-up rows,
+  8-bit activation checkpoints and the gradients that read them;
 * :mod:`.parallel` - process-group bootstrap and GPU placement;
 * :mod:`.utils` - timing, events, environment helpers.
 """
