@@ -41,7 +41,8 @@ template <> struct RowReader<kE4m3> {
 };
 
 // Any width, stride and alignment: one block per row, which it reads three
-// times (twice from cache).
+// times (twice from cache).  What takes it: rows past 16384 columns, and codes
+// whose rows, entries or scale blocks are not whole vectors.
 template <uint32_t IN, uint32_t OUT>
 __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_constant__ NormForwardParams p) {
     __shared__ WarpSums s_sum[2];
@@ -133,7 +134,12 @@ struct RowShare {
 
 // The row is read once and held in registers between the two sums and the
 // output.  Sixteen lanes hold a checkpoint block, so its largest value takes
-// four shuffles.
+// four shuffles.  Four chunks per thread: with two, the two sums (a barrier and
+// ten shuffles each) were shared by half as many values.  8192 x 12288 bf16 with
+// 8 bits kept: 98 us, 5.1 TB/s; 4096 x 6144: 22.6 us, 4.4 TB/s; from e4m3 rows
+// 23.4 us, 3.2 TB/s.  Bound by issue slots: they are taken 45-60% of the time
+// (decoding, the parameters' conversion, sums) with 24 warps per SM, which is
+// what 80 registers allow; 64 registers and 30 warps spilled and were slower.
 template <uint32_t IN, uint32_t OUT, uint32_t PARAM, int V, bool FULL, bool FP8, int T>
 __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     norm_forward_row(const __grid_constant__ NormForwardParams p, bool warp_rows) {
@@ -294,10 +300,12 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     }
 }
 
-// Rows of 16- and 32-bit values of any width and alignment up to 16 T E columns,
-// one read: as above with single values for chunks, so every access is one
-// element (64 or 128 bytes of a warp together).  E is a multiple of four: a
-// warp's columns are whole checkpoint blocks.
+// Rows of 16- and 32-bit values of any width up to 16384 and any alignment, one
+// read: as above with single values for chunks, so every access is one element
+// (64 or 128 bytes of a warp together).  E is a multiple of four: a warp's
+// columns are whole checkpoint blocks.  4096 x 4097 bf16: 39 us, 1.7 TB/s, bound
+// by issue slots (with eight elements per thread the sums' share made it 52 us;
+// reading the row three times took 56 us).
 template <uint32_t IN, uint32_t PARAM, int E, bool FP8, int T0>
 __global__ void __launch_bounds__(T0, 1024 / T0)
     norm_forward_elements(const __grid_constant__ NormForwardParams p, bool warp_rows) {
@@ -433,8 +441,9 @@ __global__ void __launch_bounds__(kRowThreads) norm_backward_rows_any(const __gr
     }
 }
 
-// Column sums of dy and dy h over one part of the rows: a block takes 32
-// columns, its warps take every eighth row of the part.
+// Past 12288 columns of what norm_backward_row does not take: dx by a block per
+// row, then column sums of dy and dy h over one part of the rows: a block takes
+// 32 columns, its warps every eighth row of the part.
 template <uint32_t X, uint32_t DY>
 __global__ void __launch_bounds__(kRowThreads) norm_backward_columns_any(const __grid_constant__ NormBackwardParams p) {
     __shared__ float s_w[kRowWarps][32], s_b[kRowWarps][32];
@@ -490,6 +499,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
 // its sums for dweight and dbias stay in registers, and each block leaves one
 // part of them.  A ring slot holds dy's row, then the kept one, each with room
 // for a chunk in every place; what no chunk fills is zero and adds nothing.
+// Both passes over a row read it from the ring: holding it in registers beside
+// the sums left one block per SM.  8192 x 12288 from 8 bits: 96 us, 5.26 TB/s
+// (0.80 of a copy's rate); 4096 x 6144 bf16 exact: 31 us, 4.9 TB/s, 5 us of
+// them the join of the parts.
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
 __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
     constexpr int kDepth = ring_depth(DY);
@@ -523,7 +536,7 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
                                      : static_cast<const uint8_t *>(p.x) + share.row * p.x_stride * int64_t(element_bytes(X));
     const int64_t dy_step = share.step * p.dy_stride * int64_t(element_bytes(DY));
     const int64_t x_step = X == kE4m3 ? share.step * p.codes_stride : share.step * p.x_stride * int64_t(element_bytes(X));
-    const uint32_t dy_bytes = chunks * Raw8<DY>::kBytes, x_bytes = (chunks * Raw8<X>::kBytes + 15) / 16 * 16;
+    const uint32_t dy_bytes = chunks * Raw8<DY>::kBytes, x_bytes = chunks * Raw8<X>::kBytes;
     uint32_t copied = share.row;
     auto copy = [&](uint32_t slot) {  // the leader's
         if (copied < rows) {
@@ -664,7 +677,9 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
     }
 }
 
-// The same for rows of any width and alignment, by single elements.
+// The same for rows of up to 12288 columns of any alignment, by single elements.
+// 4096 x 4097 bf16: 58 us, 1.7 TB/s (two passes over the rows took 111 us); a
+// branch around each load made it 83 us, from 8 bits 192 us.
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int E, int T>
 __global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
     using D = typename Element<DY>::T;
