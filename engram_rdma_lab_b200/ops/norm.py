@@ -50,7 +50,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=N
     each looked-up row of ``hidden`` columns (default: the width); ``y`` is then ``dtype`` (default bf16).
     ``weight`` and ``bias [width]`` have y's type or are fp32.  ``keep`` says what the backward pass will read:
     nothing (``kept`` is None), ``"exact"`` (``x`` itself, which must stay unchanged) or ``"fp8"``.  Codes of a lookup
-    are kept as ``"fp8"`` only: the next fetch reuses their memory.
+    are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call
+    (:func:`layer_norm` is its form).
     """
     mode = _keep_mode(keep)
     y, codes, code_scales, mean, rstd = _native.load().norm_forward(

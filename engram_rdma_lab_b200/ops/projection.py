@@ -42,7 +42,7 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dz):
         codes, scales, weight = ctx.saved_tensors
-        dz = _adjacent(dz)
+        dz = _adjacent(dz).to(weight.dtype)  # autocast may have changed the product's type
         dx = dz @ weight if ctx.wants[0] else None
         dweight = dbias = None
         if ctx.wants[1]:
@@ -73,7 +73,7 @@ class _NormLinear(torch.autograd.Function):
     def backward(ctx, dz):
         codes, scales, rstd, norm_weight, norm_bias, weight = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dz = _adjacent(dz)
+        dz = _adjacent(dz).to(weight.dtype)  # autocast may have changed the product's type
         dx = dnw = dnb = dweight = dbias = None
         if need[0] or need[1] or need[2]:
             dx, dnw, dnb = layer_norm_backward(dz @ weight, KeptRows(codes, scales, None, rstd), norm_weight,

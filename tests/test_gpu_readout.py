@@ -557,6 +557,18 @@ def test_weight_grad_of_strided_operands():
     close(fp8_weight_grad(dy, packed, s)[0], want, t + rounded(want, BF16), "dweight")
 
 
+def test_weight_grad_rounds_values_whose_scales_are_no_powers_of_two():
+    """amax / 448 scales: a decoded value is rounded to bf16 once, half a step of it."""
+    m, n, out = 200, 300, 64
+    codes, scales = quantize_fp8_blockwise(randn(1, m, n))
+    dy = randn(2, m, out, dtype=BF16)
+    (want, t), (sums, tb) = weight_grad_exact(dy, codes, scales)
+    x = codes.double().abs() * scales.double().repeat_interleave(128, 1)[:, :n]
+    dw, db = fp8_weight_grad(dy, codes, scales, dtype=FP32)
+    close(dw, want, t + half_step(BF16) * (dy.double().abs().t() @ x) + rounded(want, FP32), "dweight")
+    close(db, sums, tb + rounded(sums, FP32), "dbias")
+
+
 def test_weight_grad_scales_far_from_one_and_non_finite_codes():
     m, n, out = 70, 256, 40
     x = randn(1, m, n) * torch.exp2(torch.randint(-60, 60, (m, 1), generator=gen(2), device="cuda").float())
@@ -587,6 +599,16 @@ def test_linear_keeps_its_input_in_8_bits(dtype):
     dx, dw, dc = torch.autograd.grad(z, (x, w, c), dz)
     want = fp8_weight_grad(dz, *save_fp8(x.detach()))
     assert torch.equal(dx, dz @ w.detach()) and torch.equal(dw, want[0]) and torch.equal(dc, want[1])
+
+
+def test_projections_under_autocast():
+    x = randn(1, 40, 256, dtype=BF16).requires_grad_()
+    w = randn(2, 32, 256, dtype=BF16).requires_grad_()
+    nw, nb = (p.requires_grad_() for p in params(256, BF16))
+    with torch.autocast("cuda", FP16):
+        z = linear(x, w) + norm_linear(x, nw, nb, w)
+    z.float().sum().backward()
+    assert all(t.grad.dtype == BF16 and torch.isfinite(t.grad).all() for t in (x, w, nw, nb))
 
 
 def test_norm_linear_is_its_parts():
