@@ -132,6 +132,15 @@ struct RowShare {
     }
 };
 
+// A wait that ran out: reported, and the ring's other copies may still land
+// before the block goes.
+__device__ __forceinline__ void give_up(uint64_t *full, int depth, uint32_t slot, uint32_t phase, bool leader, uint32_t *fault) {
+    st_release_sys_u32(fault, kPipelineTimeout);
+    if (leader)
+        for (uint32_t d = 0; d < uint32_t(depth); ++d)
+            mbar_wait_often(&full[d], d >= slot ? phase : phase ^ 1, kWaitNs);
+}
+
 // The row is read once and held in registers between the two sums and the
 // output.  Sixteen lanes hold a checkpoint block, so its largest value takes
 // four shuffles.  Four chunks per thread: with two, the two sums (a barrier and
@@ -206,7 +215,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     const bool affine = p.weight != nullptr, shifted = p.bias != nullptr;
     for (uint32_t r = share.row; r < rows; r += share.step) {
         if (!mbar_wait_often(&s_full[share.group][slot], phase, kWaitNs)) {
-            st_release_sys_u32(p.fault, kPipelineTimeout);
+            give_up(s_full[share.group], kDepth, slot, phase, share.leader, p.fault);
             return;
         }
         Pair x[V][4];
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
         if (r + share.step < rows)
             load_stats(r + share.step);
         if (!mbar_wait_often(&s_full[share.group][slot], phase, kWaitNs)) {
-            st_release_sys_u32(p.fault, kPipelineTimeout);
+            give_up(s_full[share.group], kDepth, slot, phase, share.leader, p.fault);
             return;
         }
         auto values = [&](int i, Pair (&g)[4], Pair (&h)[4]) {

@@ -228,12 +228,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64
     return true;
 }
 
-// Polls until `done`; false after `timeout_ns` (or as many polls).  The timer is
-// read once in 256 polls: a read takes as long as many of them, and a waiter
-// in the middle of one sees its barrier late.
-template <class Done> __device__ __forceinline__ bool mbar_poll(uint64_t timeout_ns, Done done) {
+// mbar_wait that reads the timer once in 256 polls (a read takes as long as many
+// of them), for waits on the critical path of a pipeline.
+__device__ __forceinline__ bool mbar_wait_often(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
     uint64_t start = 0;
-    for (uint64_t polls = 1; !done(); ++polls) {
+    for (uint64_t polls = 1; !mbar_try_wait(bar, parity); ++polls) {
         if (polls % 256 != 0)
             continue;
         const uint64_t now = global_timer_ns();
@@ -243,11 +242,6 @@ template <class Done> __device__ __forceinline__ bool mbar_poll(uint64_t timeout
             return false;
     }
     return true;
-}
-
-// mbar_wait for waits on the critical path of a pipeline.
-__device__ __forceinline__ bool mbar_wait_often(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
-    return mbar_poll(timeout_ns, [&] { return mbar_try_wait(bar, parity); });
 }
 
 // Non-multicast bulk copy global -> this CTA's shared memory, completing

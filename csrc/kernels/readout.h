@@ -56,7 +56,7 @@ struct NormBackwardParams {
     uint32_t *fault;         // host-mapped: set when a wait ran out
     int64_t rows, dy_stride, x_stride, codes_stride, code_scales_stride, scale_col_stride;
     uint32_t width, parts;
-    uint32_t dy_type, x_type, param_type, keep;
+    uint32_t dy_type, param_type, keep;
 };
 
 struct SaveFp8Params {

@@ -199,7 +199,7 @@ template <> struct RowSums<768> : WideSums {};
 template <> struct RowSums<1024> : WideSums {};
 
 // Eight adjacent values as they lie in memory: 16 bytes of a 16-bit type, 32
-// of fp32, 8 of codes.  Rows are streamed past L1; parameters stay in it.
+// of fp32, 8 of codes.
 template <uint32_t TYPE> struct Raw8 {
     Vec16 v;
     static constexpr int kBytes = 16;
@@ -212,20 +212,6 @@ template <> struct Raw8<kE4m3> {
     uint2 v;
     static constexpr int kBytes = 8;
 };
-
-template <uint32_t TYPE> __device__ __forceinline__ Raw8<TYPE> load_row8(const void *ptr) {
-    Raw8<TYPE> r;
-    if constexpr (TYPE == kE4m3) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.v.x), "=r"(r.v.y) : "l"(ptr));
-    } else if constexpr (TYPE == kFp32) {
-        const Vec32 w = ld_nc_na_v8(ptr);
-        r.v = Vec16{w.v[0], w.v[1], w.v[2], w.v[3]};
-        r.v2 = Vec16{w.v[4], w.v[5], w.v[6], w.v[7]};
-    } else {
-        r.v = ld_nc_na_v4(ptr);
-    }
-    return r;
-}
 
 // Two fp32 values in one register pair, and two operations in one instruction
 // (sm_100).  The kernels over rows are bound by issue slots as much as by

@@ -271,7 +271,6 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
     p.dy_stride = dy.stride(0);
     p.width = uint32_t(width);
     p.dy_type = element_type(dy.scalar_type());
-    p.x_type = element_type(kept.scalar_type());
     p.param_type = weight ? element_type(weight->scalar_type()) : 0;
     p.keep = fp8 ? kKeepFp8 : kKeepStats;
     p.fault = healthy_word(device);
