@@ -489,10 +489,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x * 32 + lane;
     const float *partial = p.partial + int64_t(blockIdx.y) * p.parts * p.width + c;
     float sum = 0.f;
+    wait_for_previous();
     if (c < p.width)
 #pragma unroll 8
         for (uint32_t part = warp; part < p.parts; part += kJoinWarps)
-            sum += __ldg(partial + int64_t(part) * p.width);
+            sum += partial[int64_t(part) * p.width];
     s_sum[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && c < p.width) {
@@ -653,6 +654,7 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
     }
     if (p.dweight == nullptr)
         return;
+    start_next();
     float *part[2] = {p.partial + int64_t(blockIdx.x) * p.width, p.partial + int64_t(p.parts + blockIdx.x) * p.width};
     if (!warp_rows) {
 #pragma unroll
@@ -753,6 +755,7 @@ __global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(cons
     }
     if (p.dweight == nullptr)
         return;
+    start_next();
     float *part[2] = {p.partial + int64_t(blockIdx.x) * p.width, p.partial + int64_t(p.parts + blockIdx.x) * p.width};
     if (!warp_rows) {
 #pragma unroll
@@ -952,7 +955,7 @@ cudaError_t backward(const NormBackwardParams &p, int num_sms, cudaStream_t stre
             norm_backward_columns_any<X, DY><<<dim3((p.width + 31) / 32, p.parts), kRowThreads, 0, stream>>>(p);
     }
     if (rc == cudaSuccess && p.dweight != nullptr)
-        norm_backward_join<<<dim3((p.width + 31) / 32, 2), kJoinWarps * 32, 0, stream>>>(p);
+        rc = launch_overlapped(norm_backward_join, dim3((p.width + 31) / 32, 2), kJoinWarps * 32, 0, stream, p);
     return rc;
 }
 

@@ -343,6 +343,29 @@ template <uint32_t TYPE> __device__ __forceinline__ void load_shared8(uint32_t a
     unpack8<TYPE>(r, x);
 }
 
+// A kernel that only needs the one before it in its stream for a part of its
+// work starts while that one ends: the earlier one says when (all its blocks
+// have called start_next or ended), the later one waits for its end and its
+// memory where it needs them.
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... Params, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t shared, cudaStream_t stream,
+                              const Args &...args) {
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 inline bool on_boundary(const void *ptr, uint32_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes == 0; }
 
 inline __host__ __device__ constexpr uint32_t element_bytes(uint32_t type) { return type == kFp32 ? 4 : type == kE4m3 ? 1 : 2; }

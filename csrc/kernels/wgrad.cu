@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kThreads) dy_sums_part(const __grid_constant__
     const int64_t share = (p.rows + p.sum_rows - 1) / p.sum_rows;
     const int64_t first = int64_t(blockIdx.y) * share, last = min(first + share, p.rows);
     float sum[W] = {};
+    start_next();
     if (o < p.out)
 #pragma unroll 8
         for (int64_t r = first + warp; r < last; r += kThreads / 32) {
@@ -436,6 +437,7 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
             s.bias[c] = shifted && there ? load_param(p.norm_bias, p.param_type, tile_k0 + c) : 0.f;
         }
         const bool told = tile_k0 == 0 && part == 0;  // to the join and the bias
+        wait_for_previous();  // the sums' parts; nothing else here needs them
         if (p.dy_sums != nullptr && (shifted || told)) {
             // A lane's eight outputs together: their loads are in flight at once.
             float sum[8] = {};
@@ -590,19 +592,20 @@ CUtensorMap tile_map(CUtensorMapDataType type, const void *base, uint64_t column
 
 template <uint32_t TYPE> void dy_passes(const WeightGradParams &p, cudaStream_t stream) {
     constexpr int kVector = 16 / element_bytes(TYPE);
-    if (p.dy_sums != nullptr) {
-        if (on_boundary(p.dy, 16) && p.dy_stride % kVector == 0 && p.out % kVector == 0)
-            dy_sums_part<TYPE, kVector>
-                <<<dim3((p.out + 32 * kVector - 1) / (32 * kVector), p.sum_rows), kThreads, 0, stream>>>(p);
-        else
-            dy_sums_part<TYPE, 1><<<dim3((p.out + 31) / 32, p.sum_rows), kThreads, 0, stream>>>(p);
-    }
     if (p.dy_planes != nullptr) {
         const dim3 grid((p.out + 255) / 256, uint32_t(std::min<int64_t>((p.rows + 3) / 4, 4096)));
         if (on_boundary(p.dy, 16) && p.dy_stride % 4 == 0 && p.out % 4 == 0)
             split_dy<TYPE, true><<<grid, kThreads, 0, stream>>>(p);
         else
             split_dy<TYPE, false><<<grid, kThreads, 0, stream>>>(p);
+    }
+    // Last, so that the product overlaps this alone.
+    if (p.dy_sums != nullptr) {
+        if (on_boundary(p.dy, 16) && p.dy_stride % kVector == 0 && p.out % kVector == 0)
+            dy_sums_part<TYPE, kVector>
+                <<<dim3((p.out + 32 * kVector - 1) / (32 * kVector), p.sum_rows), kThreads, 0, stream>>>(p);
+        else
+            dy_sums_part<TYPE, 1><<<dim3((p.out + 31) / 32, p.sum_rows), kThreads, 0, stream>>>(p);
     }
 }
 
@@ -668,8 +671,14 @@ cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
     cudaError_t rc = cudaFuncSetAttribute(weight_grad_tensor, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess)
         return rc;
-    weight_grad_tensor<<<2 * p.tiles_o * p.tiles_k * p.parts, kTensorThreads, kSharedBytes, stream>>>(q, dy_map, code_map,
-                                                                                                     out_map);
+    const dim3 grid(2 * p.tiles_o * p.tiles_k * p.parts);
+    if (p.dy_sums != nullptr) {
+        rc = launch_overlapped(weight_grad_tensor, grid, kTensorThreads, kSharedBytes, stream, q, dy_map, code_map, out_map);
+        if (rc != cudaSuccess)
+            return rc;
+    } else {
+        weight_grad_tensor<<<grid, kTensorThreads, kSharedBytes, stream>>>(q, dy_map, code_map, out_map);
+    }
     if (p.parts > 1) {
         const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
         weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(p);
