@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
 // part of them.  A ring slot holds dy's row, then the kept one, each with room
 // for a chunk in every place; what no chunk fills is zero and adds nothing.
 // Both passes over a row read it from the ring: holding it in registers beside
-// the sums left one block per SM.  8192 x 12288 from 8 bits: 96 us, 5.26 TB/s
-// (0.80 of a copy's rate); 4096 x 6144 bf16 exact: 31 us, 4.9 TB/s, 5 us of
+// the sums left one block per SM.  8192 x 12288 from 8 bits: 94 us, 5.33 TB/s
+// (0.81 of a copy's rate); 4096 x 6144 bf16 exact: 31 us, 4.9 TB/s, 4-5 us of
 // them the join of the parts.
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
 __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
