@@ -5,7 +5,8 @@
 // h mean(g h)); per column: dw = sum dy h, db = sum dy.  All sums are fp32.
 // The variance is the corrected two-pass form: with d = x - m for the first
 // pass's mean m, sum d (zero but for m's rounding) corrects both mean and
-// variance, so a large common offset of a row costs no digits.
+// variance, so a large common offset of a row costs no digits as long as m and
+// the correction are taken off one after the other: their sum rounds.
 #include <algorithm>
 
 #include "readout.h"
@@ -66,10 +67,9 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
         const float2 sums = block_sum2(a, b, s_sum[1]);
         const float shift = sums.x * inv;
         const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
-        mean += shift;
         if (threadIdx.x == 0) {
             if (p.keep == kKeepStats)
-                p.mean[r] = mean;
+                p.mean[r] = mean + shift;
             if (p.keep != kKeepNothing)
                 p.rstd[r] = rstd;
         }
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
                 const uint32_t c = blk * kCheckpointBlock + i * 32 + lane;
                 h[i] = 0.f;
                 if (c < p.width) {
-                    h[i] = (x(c) - mean) * rstd;
+                    h[i] = (x(c) - mean - shift) * rstd;
                     amax = fmaxf(amax, finite_abs(h[i]));
                     float v = h[i];
                     if (p.weight != nullptr)
