@@ -17,7 +17,7 @@ constexpr uint32_t kCheckpointBlock = 128;
 // What a forward norm keeps for its backward pass.
 enum KeepMode : uint32_t {
     kKeepNothing = 0,
-    kKeepStats = 1,  // mean and rstd; the caller keeps the rows
+    kKeepStats = 1,  // mean (in two parts) and rstd; the caller keeps the rows
     kKeepFp8 = 2,    // rstd and the normalised rows in 8 bits
 };
 
@@ -30,7 +30,8 @@ struct NormForwardParams {
     const void *weight;      // nullptr: no affine part
     const void *bias;        // nullptr: none
     void *y;
-    float *mean, *rstd;      // [rows]; mean with kKeepStats, rstd with either
+    float *mean, *shift;     // [rows], kKeepStats: the mean is their sum, shift what mean's rounding left
+    float *rstd;             // [rows], with either
     uint8_t *codes;          // kKeepFp8: [rows][codes_stride]
     float *code_scales;      // kKeepFp8: [rows][ceil(width / 128)]
     uint32_t *fault;         // host-mapped: set when a wait ran out
@@ -41,12 +42,12 @@ struct NormForwardParams {
 };
 
 // dx, and per-column sums for dweight and dbias.  The normalised rows come from
-// `x`, `mean` and `rstd` (kKeepStats; x as above) or from `codes` and
+// `x`, `mean`, `shift` and `rstd` (kKeepStats; x as above) or from `codes` and
 // `code_scales` (kKeepFp8).
 struct NormBackwardParams {
     const void *dy;
     const void *x;
-    const float *mean, *rstd;
+    const float *mean, *shift, *rstd;  // shift nullptr: zeros
     const uint8_t *codes;
     const float *code_scales;
     const void *weight;      // nullptr: no affine part

@@ -141,7 +141,7 @@ uint32_t *healthy_word(int device) {
     return word;
 }
 
-// (y, codes | None, scales | None, mean | None, rstd | None)
+// (y, codes | None, scales | None, mean | None, rstd | None, shift | None)
 py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps,
                        const OptTensor &scales, std::optional<int64_t> hidden, int64_t block,
                        std::optional<ScalarType> dtype, uint32_t keep) {
@@ -177,11 +177,13 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
     const int device = need_device(x, {&weight, &bias, &scales});
     c10::cuda::CUDAGuard guard(device);
     const Tensor y = empty({rows, width}, out, x);
-    OptTensor codes, code_scales, mean, rstd;
+    OptTensor codes, code_scales, mean, rstd, shift;
     if (keep != kKeepNothing)
         rstd = empty({rows}, ScalarType::Float, x);
-    if (keep == kKeepStats)
+    if (keep == kKeepStats) {
         mean = empty({rows}, ScalarType::Float, x);
+        shift = empty({rows}, ScalarType::Float, x);
+    }
     if (keep == kKeepFp8) {
         codes = empty_codes(x, rows, width);
         code_scales = empty_scales(x, rows, width);
@@ -192,6 +194,7 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
         p.bias = data(bias);
         p.y = y.data_ptr();
         p.mean = static_cast<float *>(data(mean));
+        p.shift = static_cast<float *>(data(shift));
         p.rstd = static_cast<float *>(data(rstd));
         p.codes = static_cast<uint8_t *>(data(codes));
         p.code_scales = static_cast<float *>(data(code_scales));
@@ -208,12 +211,13 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
         check_cuda(launch_norm_forward(p, sm_count(device), at::cuda::getCurrentCUDAStream(device).stream()),
                    "launch layer norm");
     }
-    return py::make_tuple(y, codes, code_scales, mean, rstd);
+    return py::make_tuple(y, codes, code_scales, mean, rstd, shift);
 }
 
-// (dx | None, dweight | None, dbias | None).  Kept rows: (x, mean, rstd) or (codes, scales, rstd).
+// (dx | None, dweight | None, dbias | None).  Kept rows: (x, mean, rstd, shift | None) or (codes, scales, rstd).
 py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &scales, const OptTensor &mean,
-                        const Tensor &rstd, const OptTensor &weight, bool want_dx, bool want_params) {
+                        const Tensor &rstd, const OptTensor &weight, bool want_dx, bool want_params,
+                        const OptTensor &shift) {
     need_rows(dy, "dy must be [tokens, width] with adjacent columns");
     need(is_wide(dy.scalar_type()), "dy must be bfloat16, float16 or float32");
     const int64_t rows = dy.size(0), width = dy.size(1);
@@ -227,12 +231,15 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
         need(mean && mean->dim() == 1 && mean->size(0) == rows && mean->scalar_type() == ScalarType::Float &&
                  mean->is_contiguous(),
              "mean must be contiguous float32 [tokens]");
+        need(!shift || (shift->dim() == 1 && shift->size(0) == rows && shift->scalar_type() == ScalarType::Float &&
+                        shift->is_contiguous()),
+             "shift must be contiguous float32 [tokens]");
     }
     need(rstd.dim() == 1 && rstd.size(0) == rows && rstd.scalar_type() == ScalarType::Float && rstd.is_contiguous(),
          "rstd must be contiguous float32 [tokens]");
     need_params(weight, std::nullopt, width, dy.scalar_type());
     const OptTensor kept_opt = kept, rstd_opt = rstd;
-    const int device = need_device(dy, {&kept_opt, &scales, &mean, &rstd_opt, &weight});
+    const int device = need_device(dy, {&kept_opt, &scales, &mean, &rstd_opt, &weight, &shift});
     c10::cuda::CUDAGuard guard(device);
     OptTensor dx, dweight, dbias, partial;
     if (want_dx)
@@ -262,6 +269,7 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
         p.x = kept.data_ptr();
         p.x_stride = kept.stride(0);
         p.mean = static_cast<const float *>(mean->data_ptr());
+        p.shift = static_cast<const float *>(data(shift));
     }
     p.weight = data(weight);
     p.dx = data(dx);
@@ -409,7 +417,7 @@ void bind_readout(py::module_ &m) {
     m.def("norm_forward", &norm_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),
           py::arg("scales"), py::arg("hidden"), py::arg("block"), py::arg("dtype"), py::arg("keep"));
     m.def("norm_backward", &norm_backward, py::arg("dy"), py::arg("kept"), py::arg("scales"), py::arg("mean"),
-          py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"));
+          py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"), py::arg("shift"));
     m.def(
         "debug_readout_fault",
         [](int device, uint32_t code) { return std::exchange(*static_cast<volatile uint32_t *>(fault_word(device)), code); },

@@ -2,7 +2,7 @@
 
 The rows are what a lookup returns: ``[tokens, width]`` bf16 (fp16 and fp32 work too), or e4m3 codes with their
 scales, which the kernel multiplies in as it reads (no dequantised copy).  The backward pass reads what the forward
-pass kept: the rows themselves with two fp32 numbers per row (``keep="exact"``), or the normalised rows in 8 bits
+pass kept: the rows themselves with three fp32 numbers per row (``keep="exact"``), or the normalised rows in 8 bits
 with one (``keep="fp8"``; the format of :mod:`.checkpoint`), half of bf16's bytes.  Normalised values are what suits
 8 bits: a row's common offset and size are gone before the rounding, so e4m3's relative precision is spent on what
 the gradient needs, and the same checkpoint serves the projection behind the norm
@@ -26,12 +26,17 @@ _KEEP = {None: 0, "exact": 1, "fp8": 2}
 
 
 class KeptRows(NamedTuple):
-    """What ``layer_norm_forward`` keeps: ``(x, None, mean, rstd)`` or ``(codes, scales, None, rstd)``."""
+    """What ``layer_norm_forward`` keeps: ``(x, None, mean, rstd, shift)`` or ``(codes, scales, None, rstd)``.
+
+    A row's mean is ``mean + shift``: the rounded mean, and what its rounding left (None: zeros), which counts where a
+    row's offset is many times its deviation.
+    """
 
     rows: torch.Tensor
     scales: Optional[torch.Tensor]
     mean: Optional[torch.Tensor]
     rstd: torch.Tensor
+    shift: Optional[torch.Tensor] = None
 
 
 def _keep_mode(keep) -> int:
@@ -54,11 +59,11 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=N
     (:func:`layer_norm` is its form).
     """
     mode = _keep_mode(keep)
-    y, codes, code_scales, mean, rstd = _native.load().norm_forward(
+    y, codes, code_scales, mean, rstd, shift = _native.load().norm_forward(
         x, weight, bias, eps, scales, hidden, block, dtype, mode)
     if mode == 0:
         return y, None
-    return y, KeptRows(x, None, mean, rstd) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
+    return y, KeptRows(x, None, mean, rstd, shift) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
 
 
 def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True, want_params: bool = True):
@@ -67,7 +72,8 @@ def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True
     ``dx`` has dy's type (for looked-up codes it is the gradient of the dequantised rows), ``dweight`` and ``dbias``
     the weight's type; both are None without a ``weight``.  What is not wanted is None and not computed.
     """
-    return _native.load().norm_backward(dy, kept.rows, kept.scales, kept.mean, kept.rstd, weight, want_dx, want_params)
+    return _native.load().norm_backward(dy, kept.rows, kept.scales, kept.mean, kept.rstd, weight, want_dx, want_params,
+                                        kept.shift)
 
 
 def _adjacent(t: torch.Tensor) -> torch.Tensor:
@@ -90,9 +96,9 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        rows, scales, mean, rstd, weight = ctx.saved_tensors
+        *kept, weight = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dweight, dbias = layer_norm_backward(_adjacent(dy), KeptRows(rows, scales, mean, rstd), weight,
+        dx, dweight, dbias = layer_norm_backward(_adjacent(dy), KeptRows(*kept), weight,
                                                  want_dx=need[0], want_params=need[1] or need[2])
         return dx, dweight if need[1] else None, dbias if need[2] else None, None, None, None, None, None, None
 

@@ -7,8 +7,9 @@ half a step at 4096, in every value of a row.
 """
 
 import pytest
+import torch
 
-from engram_rdma_lab_b200.ops import layer_norm_forward
+from engram_rdma_lab_b200.ops import KeptRows, layer_norm, layer_norm_backward, layer_norm_forward
 
 from .test_gpu_readout import DEPTH, EPS, FP32, U, _gpu, close, norm_exact, params, randn, rounded  # noqa: F401
 
@@ -37,3 +38,50 @@ def test_forward_of_rows_far_from_zero(n):
     y, _ = layer_norm_forward(x, w, b, EPS)
     t = h_tolerance(x, h, rstd) * w.double().abs() + 2 * U * ((h * w.double()).abs() + b.double().abs())
     close(y, want, t + rounded(want, FP32), "y")
+
+
+@pytest.mark.parametrize("n", WIDTHS)
+def test_backward_of_exact_rows_far_from_zero(n):
+    m = 64
+    x, dy = rows_far_from_zero(m, n), randn(n + 1, m, n)
+    w, b = params(n, FP32)
+    _, h, _, rstd = norm_exact(x, w, b)
+    th = h_tolerance(x, h, rstd)
+    _, kept = layer_norm_forward(x, w, b, EPS, keep="exact")
+    dx, dw, db = layer_norm_backward(dy, kept, w)
+    g = dy.double() * w.double()
+    c1, c2 = g.mean(1, keepdim=True), (g * h).mean(1, keepdim=True)
+    t1 = DEPTH * U * g.abs().mean(1, keepdim=True)
+    t2 = DEPTH * U * (g * h).abs().mean(1, keepdim=True) + (g.abs() * th).mean(1, keepdim=True)
+    want = rstd[:, None] * (g - c1 - h * c2)
+    t = rstd[:, None] * (t1 + t2 * h.abs() + th * c2.abs() + 6 * U * (g.abs() + c1.abs() + (h * c2).abs()))
+    close(dx, want, t + (DEPTH / 2 + 8) * U * want.abs() + rounded(want, FP32), "dx")
+    # A column's sum: no term goes through more additions than there are rows.
+    dy64, want = dy.double(), (dy.double() * h).sum(0)
+    t = (dy64.abs() * (th + 2 * U * h.abs())).sum(0) + m * U * (dy64 * h).abs().sum(0)
+    close(dw, want, t + rounded(want, FP32), "dweight")
+    close(db, dy64.sum(0), m * U * dy64.abs().sum(0) + rounded(dy64.sum(0), FP32), "dbias")
+
+
+def test_autograd_reads_what_the_forward_pass_kept():
+    x, dy = rows_far_from_zero(20, 1000), randn(3, 20, 1000)
+    w, b = params(1000, FP32)
+    _, kept = layer_norm_forward(x, w, b, EPS, keep="exact")
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(layer_norm(*leaves, EPS, keep="exact"), leaves, dy)
+    assert all(torch.equal(a, c) for a, c in zip(got, layer_norm_backward(dy, kept, w)))
+
+
+def test_a_single_mean_per_row_still_serves():
+    """Statistics of another origin: rows, one fp32 mean and one rstd per row."""
+    x, dy = randn(1, 30, 768), randn(2, 30, 768)
+    w, _ = params(768, FP32)
+    _, h, mean, rstd = norm_exact(x)
+    kept = KeptRows(x, None, mean.float(), rstd.float())
+    dx, dw, _ = layer_norm_backward(dy, kept, w)
+    # x - mean: the mean's rounding and the difference's, 2 U of 8 (no value is larger), rstd's rounding and the product's.
+    dh = 16 * U * rstd[:, None] + 4 * U * h.abs()
+    dy64 = dy.double()
+    t = (dy64.abs() * dh).sum(0) + 30 * U * (dy64 * h).abs().sum(0)
+    close(dw, (dy64 * h).sum(0), t + rounded((dy64 * h).sum(0), FP32), "dweight")
+    assert torch.isfinite(dx).all()
