@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native
@@ -55,8 +56,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=N
     each looked-up row of ``hidden`` columns (default: the width); ``y`` is then ``dtype`` (default bf16).
     ``weight`` and ``bias [width]`` have y's type or are fp32.  ``keep`` says what the backward pass will read:
     nothing (``kept`` is None), ``"exact"`` (``x`` itself, which must stay unchanged) or ``"fp8"``.  Codes of a lookup
-    are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call
-    (:func:`layer_norm` is its form).
+    are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call, in
+    either mode (:func:`layer_norm` is its form).
     """
     mode = _keep_mode(keep)
     y, codes, code_scales, mean, rstd, shift = _native.load().norm_forward(
@@ -85,6 +86,19 @@ def _no_code_gradient(x: torch.Tensor):
         raise ValueError("float8_e4m3fn rows get no gradient; layer_norm_backward gives their dequantised rows'")
 
 
+def _recorded(*tensors) -> bool:
+    """Whether autograd has to see a call: a gradient is wanted, or forward-mode differentiation carries a tangent.
+
+    The kernels' results carry no tangent, which counts as zero; the autograd functions raise instead.
+    """
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return True
+    # Without an open level there are no tangents (and asking each tensor takes as long as the call).
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in given)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, scales, hidden, block, dtype, keep):
@@ -108,11 +122,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hid
     """Differentiable layer norm of ``x [tokens, width]``; the arguments are :func:`layer_norm_forward`'s.
 
     ``keep`` (``"fp8"`` or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
-    is wanted.  Looked-up e4m3 codes get no gradient themselves (:func:`layer_norm_backward` gives their rows').
+    is wanted.  There is no forward-mode derivative (a tangent raises).  Looked-up e4m3 codes get no gradient
+    themselves (:func:`layer_norm_backward` gives their rows').
     """
     if _keep_mode(keep) == 0:
         raise ValueError('keep must be "exact" or "fp8"')
     _no_code_gradient(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _recorded(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, scales, hidden, block, dtype, keep)
     return layer_norm_forward(x, weight, bias, eps, scales=scales, hidden=hidden, block=block, dtype=dtype)[0]

@@ -1,7 +1,7 @@
 """Projections whose backward pass reads an 8-bit checkpoint of their input.
 
 ``fp8_weight_grad`` computes a projection's weight gradient from the gradient of its output and the checkpoint,
-without a dequantised copy.  ``linear`` and ``norm_linear`` are the differentiable forms: the forward product and
+without a dequantised copy (autograd does not see the call).  ``linear`` and ``norm_linear`` are the differentiable forms: the forward product and
 the input's gradient are plain matrix products; what is kept in between is the 8-bit checkpoint alone.
 ``norm_linear`` runs a layer norm in front, and one checkpoint (the normalised rows) serves both backward passes:
 with ``n = h w + b``, ``dW = dz^T n = (dz^T h) w + (sum dz) b^T``.
@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .checkpoint import save_fp8
-from .norm import KeptRows, _adjacent, _no_code_gradient, layer_norm_backward, layer_norm_forward
+from .norm import KeptRows, _adjacent, _no_code_gradient, _recorded, layer_norm_backward, layer_norm_forward
 
 
 def fp8_weight_grad(dy, codes, scales, norm_weight=None, norm_bias=None, *, dtype=None, bias_grad: bool = True):
@@ -90,13 +90,13 @@ def norm_linear(x, norm_weight, norm_bias, weight, bias=None, eps: float = 1e-5,
     """Differentiable ``layer_norm(x) @ weight^T + bias`` that keeps only the normalised rows, in 8 bits.
 
     ``x``, ``scales``, ``hidden``, ``block`` and ``dtype`` are :func:`~.norm.layer_norm_forward`'s; ``weight
-    [features, width]`` and ``bias [features]`` have the type of the normalised rows.
+    [features, width]`` and ``bias [features]`` have the type of the normalised rows.  There is no forward-mode
+    derivative (a tangent raises).
     """
     _no_code_gradient(x)
     out = (dtype or torch.bfloat16) if x.dtype == torch.float8_e4m3fn else x.dtype
     _check_projection(out, x, weight, bias)
-    tensors = (x, norm_weight, norm_bias, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _recorded(x, norm_weight, norm_bias, weight, bias):
         return _NormLinear.apply(x, norm_weight, norm_bias, weight, bias, eps, scales, hidden, block, dtype)
     normed, _ = layer_norm_forward(x, norm_weight, norm_bias, eps, scales=scales, hidden=hidden, block=block,
                                    dtype=dtype)
