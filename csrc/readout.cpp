@@ -3,6 +3,7 @@
 // Arguments are checked here (ValueError, before any device is touched);
 // everything runs on the current stream of the inputs' device, and outputs and
 // workspaces come from torch's allocator, so calls can be captured into graphs.
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -33,6 +34,14 @@ using OptTensor = std::optional<Tensor>;
 void need(bool ok, const char *what) {
     if (!ok)
         throw py::value_error(what);
+}
+
+// A trace (torch.jit.trace) does not see these calls and would keep their results
+// as constants.  `recorded`: the caller is an autograd function, which a trace
+// records as a whole.
+void need_untraced(bool recorded) {
+    check(recorded || !at::tracer::impl::is_dispatch_enabled(),
+          "a trace would keep this call's result as a constant; trace layer_norm, linear or norm_linear");
 }
 
 bool is_wide(ScalarType t) {
@@ -144,7 +153,8 @@ uint32_t *healthy_word(int device) {
 // (y, codes | None, scales | None, mean | None, rstd | None, shift | None)
 py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps,
                        const OptTensor &scales, std::optional<int64_t> hidden, int64_t block,
-                       std::optional<ScalarType> dtype, uint32_t keep) {
+                       std::optional<ScalarType> dtype, uint32_t keep, bool recorded) {
+    need_untraced(recorded);
     need_rows(x, "rows must be [tokens, width] with adjacent columns");
     const int64_t rows = x.size(0), width = x.size(1);
     const bool fp8 = x.scalar_type() == ScalarType::Float8_e4m3fn;
@@ -218,6 +228,7 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
 py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &scales, const OptTensor &mean,
                         const Tensor &rstd, const OptTensor &weight, bool want_dx, bool want_params,
                         const OptTensor &shift) {
+    need_untraced(false);
     need_rows(dy, "dy must be [tokens, width] with adjacent columns");
     need(is_wide(dy.scalar_type()), "dy must be bfloat16, float16 or float32");
     const int64_t rows = dy.size(0), width = dy.size(1);
@@ -293,7 +304,8 @@ py::tuple norm_backward(const Tensor &dy, const Tensor &kept, const OptTensor &s
     return py::make_tuple(dx, dweight, dbias);
 }
 
-py::tuple save_fp8(const Tensor &x) {
+py::tuple save_fp8(const Tensor &x, bool recorded) {
+    need_untraced(recorded);
     need_rows(x, "activations must be [rows, width] with adjacent columns");
     need(is_wide(x.scalar_type()), "activations must be bfloat16, float16 or float32");
     const int device = need_device(x, {});
@@ -317,6 +329,7 @@ py::tuple save_fp8(const Tensor &x) {
 }
 
 Tensor restore_fp8(const Tensor &codes, const Tensor &scales, ScalarType dtype) {
+    need_untraced(false);
     need_checkpoint(codes, scales);
     need(is_wide(dtype), "dtype must be bfloat16, float16 or float32");
     const OptTensor scales_opt = scales;
@@ -344,6 +357,7 @@ Tensor restore_fp8(const Tensor &codes, const Tensor &scales, ScalarType dtype) 
 // (dweight [out, width], dbias [out] | None)
 py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &scales, const OptTensor &norm_weight,
                           const OptTensor &norm_bias, std::optional<ScalarType> dtype, bool want_bias) {
+    need_untraced(false);
     need_rows(dy, "dy must be [rows, out] with adjacent columns");
     need(is_wide(dy.scalar_type()), "dy must be bfloat16, float16 or float32");
     need_checkpoint(codes, scales);
@@ -415,14 +429,15 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
 
 void bind_readout(py::module_ &m) {
     m.def("norm_forward", &norm_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"),
-          py::arg("scales"), py::arg("hidden"), py::arg("block"), py::arg("dtype"), py::arg("keep"));
+          py::arg("scales"), py::arg("hidden"), py::arg("block"), py::arg("dtype"), py::arg("keep"),
+          py::arg("recorded") = false);
     m.def("norm_backward", &norm_backward, py::arg("dy"), py::arg("kept"), py::arg("scales"), py::arg("mean"),
           py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"), py::arg("shift"));
     m.def(
         "debug_readout_fault",
         [](int device, uint32_t code) { return std::exchange(*static_cast<volatile uint32_t *>(fault_word(device)), code); },
         py::arg("device"), py::arg("code"), "Replace a device's fault word (tests of how a given-up wait is reported).");
-    m.def("save_fp8", &save_fp8, py::arg("x"));
+    m.def("save_fp8", &save_fp8, py::arg("x"), py::arg("recorded") = false);
     m.def("restore_fp8", &restore_fp8, py::arg("codes"), py::arg("scales"), py::arg("dtype"));
     m.def("fp8_weight_grad", &fp8_weight_grad, py::arg("dy"), py::arg("codes"), py::arg("scales"),
           py::arg("norm_weight"), py::arg("norm_bias"), py::arg("dtype"), py::arg("want_bias"));

@@ -47,6 +47,15 @@ def _keep_mode(keep) -> int:
         raise ValueError('keep must be None, "exact" or "fp8"') from None
 
 
+def _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, recorded):
+    mode = _keep_mode(keep)
+    y, codes, code_scales, mean, rstd, shift = _native.load().norm_forward(
+        x, weight, bias, eps, scales, hidden, block, dtype, mode, recorded)
+    if mode == 0:
+        return y, None
+    return y, KeptRows(x, None, mean, rstd, shift) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
+
+
 def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hidden=None, block: int = 128,
                        dtype=None, keep=None):
     """``(y, kept)`` with ``y = (x - mean) / sqrt(var + eps) * weight + bias`` for each row of ``x [tokens, width]``.
@@ -57,14 +66,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=N
     ``weight`` and ``bias [width]`` have y's type or are fp32.  ``keep`` says what the backward pass will read:
     nothing (``kept`` is None), ``"exact"`` (``x`` itself, which must stay unchanged) or ``"fp8"``.  Codes of a lookup
     are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call, in
-    either mode (:func:`layer_norm` is its form).
+    either mode, nor does a trace, which is refused (:func:`layer_norm` is their form).
     """
-    mode = _keep_mode(keep)
-    y, codes, code_scales, mean, rstd, shift = _native.load().norm_forward(
-        x, weight, bias, eps, scales, hidden, block, dtype, mode)
-    if mode == 0:
-        return y, None
-    return y, KeptRows(x, None, mean, rstd, shift) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
+    return _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, False)
 
 
 def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True, want_params: bool = True):
@@ -87,12 +91,14 @@ def _no_code_gradient(x: torch.Tensor):
 
 
 def _recorded(*tensors) -> bool:
-    """Whether autograd has to see a call: a gradient is wanted, or forward-mode differentiation carries a tangent.
+    """Whether autograd has to see a call: a gradient is wanted, a trace records, or forward-mode differentiation
+    carries a tangent.
 
-    The kernels' results carry no tangent, which counts as zero; the autograd functions raise instead.
+    The kernels' results carry no tangent, which counts as zero (the autograd functions raise instead), and a trace
+    takes them as constants (it records an autograd function as one operation).
     """
     given = [t for t in tensors if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given) or torch.jit.is_tracing():
         return True
     # Without an open level there are no tangents (and asking each tensor takes as long as the call).
     return getattr(forward_ad, "_current_level", 0) >= 0 and any(
@@ -102,8 +108,7 @@ def _recorded(*tensors) -> bool:
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, scales, hidden, block, dtype, keep):
-        y, kept = layer_norm_forward(x, weight, bias, eps, scales=scales, hidden=hidden, block=block, dtype=dtype,
-                                     keep=keep)
+        y, kept = _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, True)
         ctx.save_for_backward(*kept, weight)
         return y
 

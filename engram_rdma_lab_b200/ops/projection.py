@@ -1,8 +1,9 @@
 """Projections whose backward pass reads an 8-bit checkpoint of their input.
 
 ``fp8_weight_grad`` computes a projection's weight gradient from the gradient of its output and the checkpoint,
-without a dequantised copy (autograd does not see the call).  ``linear`` and ``norm_linear`` are the differentiable forms: the forward product and
-the input's gradient are plain matrix products; what is kept in between is the 8-bit checkpoint alone.
+without a dequantised copy (autograd does not see the call, and a trace is refused).  ``linear`` and ``norm_linear``
+are the differentiable forms: the forward product and the input's gradient are plain matrix products; what is kept in
+between is the 8-bit checkpoint alone.
 ``norm_linear`` runs a layer norm in front, and one checkpoint (the normalised rows) serves both backward passes:
 with ``n = h w + b``, ``dW = dz^T n = (dz^T h) w + (sum dz) b^T``.
 """
@@ -13,8 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native
-from .checkpoint import save_fp8
-from .norm import KeptRows, _adjacent, _no_code_gradient, _recorded, layer_norm_backward, layer_norm_forward
+from .norm import KeptRows, _adjacent, _forward, _no_code_gradient, _recorded, layer_norm_backward, layer_norm_forward
 
 
 def fp8_weight_grad(dy, codes, scales, norm_weight=None, norm_bias=None, *, dtype=None, bias_grad: bool = True):
@@ -34,7 +34,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         ctx.wants = ctx.needs_input_grad
-        kept = save_fp8(x) if ctx.wants[1] else (None, None)
+        kept = _native.load().save_fp8(x, True) if ctx.wants[1] else (None, None)
         ctx.save_for_backward(*kept, weight)
         return torch.nn.functional.linear(x, weight, bias)
 
@@ -63,8 +63,7 @@ def linear(x, weight, bias=None):
 class _NormLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, norm_weight, norm_bias, weight, bias, eps, scales, hidden, block, dtype):
-        normed, kept = layer_norm_forward(x, norm_weight, norm_bias, eps, scales=scales, hidden=hidden, block=block,
-                                          dtype=dtype, keep="fp8")
+        normed, kept = _forward(x, norm_weight, norm_bias, eps, scales, hidden, block, dtype, "fp8", True)
         ctx.save_for_backward(kept.rows, kept.scales, kept.rstd, norm_weight, norm_bias, weight)
         return torch.nn.functional.linear(normed, weight, bias)
 

@@ -4,6 +4,9 @@ A stand-in computes what the kernels do from elementary operations on the CPU.  
 new tensors that autograd knows nothing of: no history, no tangent, and a trace sees them as constants.
 """
 
+import functools
+import threading
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -13,56 +16,68 @@ from engram_rdma_lab_b200 import _native, ops
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
+def unseen(function):
+    """Run in a thread of its own, where no trace, autocast or gradient mode of the caller reaches."""
+
+    @functools.wraps(function)
+    def call(self, *args, **kwargs):
+        plain = [a.detach() if isinstance(a, torch.Tensor) else a for a in args]
+        result = []
+
+        def work():
+            with torch.no_grad():
+                result.append(function(self, *plain, **kwargs))
+
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+        return result[0]
+
+    return call
+
+
 class StandIn:
-    @staticmethod
-    def _new(t):
-        return None if t is None else torch.frombuffer(bytearray(t.detach().contiguous().view(torch.uint8).numpy().tobytes()),
-                                                       dtype=t.dtype).view(t.shape)
+    @unseen
+    def norm_forward(self, x, weight, bias, eps, scales, hidden, block, dtype, keep, recorded=False):
+        mean = x.double().mean(1, keepdim=True)
+        rstd = 1 / torch.sqrt(((x.double() - mean) ** 2).mean(1, keepdim=True) + eps)
+        h = (x.double() - mean) * rstd
+        y = h if weight is None else h * weight.double()
+        y = (y if bias is None else y + bias.double()).to(x.dtype)
+        codes, code_scales = ops.quantize_fp8_blockwise(h.float(), power_of_two=True) if keep == 2 else (None, None)
+        exact = keep == 1
+        return (y, codes, code_scales, mean[:, 0].float() if exact else None, rstd[:, 0].float() if keep else None,
+                torch.zeros(len(x)) if exact else None)
 
-    def norm_forward(self, x, weight, bias, eps, scales, hidden, block, dtype, keep):
-        with torch.no_grad():
-            x = x.detach()
-            mean = x.double().mean(1, keepdim=True)
-            rstd = 1 / torch.sqrt(((x.double() - mean) ** 2).mean(1, keepdim=True) + eps)
-            h = (x.double() - mean) * rstd
-            y = h if weight is None else h * weight.detach().double()
-            y = (y if bias is None else y + bias.detach().double()).to(x.dtype)
-            codes, code_scales = self.save_fp8(h) if keep == 2 else (None, None)
-            exact = keep == 1
-            return (self._new(y), codes, code_scales, self._new(mean[:, 0].float()) if exact else None,
-                    self._new(rstd[:, 0].float()) if keep else None, torch.zeros(len(x)) if exact else None)
-
+    @unseen
     def norm_backward(self, dy, rows, scales, mean, rstd, weight, want_dx, want_params, shift):
-        assert weight is None or weight.dtype in (dy.dtype, FP32)
-        with torch.no_grad():
-            n = dy.shape[1]
-            r = rstd.double()[:, None]
-            h = (rows.double() - mean.double()[:, None]) * r if scales is None else self._rows(rows, scales)
-            g = dy.double() if weight is None else dy.double() * weight.detach().double()
-            dx = r * (g - g.mean(1, keepdim=True) - h * (g * h).sum(1, keepdim=True) / n)
-            parameters = want_params and weight is not None
-            return (self._new(dx.to(dy.dtype)) if want_dx else None,
-                    self._new((dy.double() * h).sum(0).to(weight.dtype)) if parameters else None,
-                    self._new(dy.double().sum(0).to(weight.dtype)) if parameters else None)
+        if weight is not None and weight.dtype not in (dy.dtype, FP32):
+            raise ValueError("weight must have the rows' type or float32")
+        r = rstd.double()[:, None]
+        h = (rows.double() - mean.double()[:, None]) * r if scales is None else self.rows(rows, scales)
+        g = dy.double() if weight is None else dy.double() * weight.double()
+        dx = r * (g - g.mean(1, keepdim=True) - h * (g * h).mean(1, keepdim=True))
+        parameters = want_params and weight is not None
+        return (dx.to(dy.dtype) if want_dx else None, (dy.double() * h).sum(0).to(weight.dtype) if parameters else None,
+                dy.double().sum(0).to(weight.dtype) if parameters else None)
 
     @staticmethod
-    def _rows(codes, scales):
+    def rows(codes, scales):
         return codes.double() * scales.double().repeat_interleave(128, 1)[:, :codes.shape[1]]
 
-    def save_fp8(self, x):
-        codes, scales = ops.quantize_fp8_blockwise(x.detach().float(), power_of_two=True)
-        return codes, self._new(scales)
+    @unseen
+    def save_fp8(self, x, recorded=False):
+        return ops.quantize_fp8_blockwise(x.float(), power_of_two=True)
 
+    @unseen
     def fp8_weight_grad(self, dy, codes, scales, norm_weight, norm_bias, dtype, want_bias):
-        with torch.no_grad():
-            x = self._rows(codes, scales)
-            if norm_weight is not None:
-                x = x * norm_weight.detach().double()
-            if norm_bias is not None:
-                x = x + norm_bias.detach().double()
-            dy64 = dy.detach().double()
-            out = dtype or dy.dtype
-            return self._new((dy64.t() @ x).to(out)), self._new(dy64.sum(0).to(out)) if want_bias else None
+        x = self.rows(codes, scales)
+        if norm_weight is not None:
+            x = x * norm_weight.double()
+        if norm_bias is not None:
+            x = x + norm_bias.double()
+        out = dtype or dy.dtype
+        return (dy.double().t() @ x).to(out), dy.double().sum(0).to(out) if want_bias else None
 
 
 @pytest.fixture(autouse=True)
@@ -119,3 +134,19 @@ def test_linear_carries_tangents():
     with forward_ad.dual_level():
         y = ops.linear(forward_ad.make_dual(x, tangent), w, b)
         torch.testing.assert_close(forward_ad.unpack_dual(y).tangent, tangent @ w.t())
+
+
+# ---------------------------------------------------------------- tracing
+@pytest.mark.filterwarnings("ignore::DeprecationWarning", "ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_trace_computes_with_its_own_inputs(form, grad):
+    call, _ = FORMS[form]
+    first = [t.requires_grad_(grad) for t in leaves()]
+    if grad and form != "norm_linear":  # torch traces no function whose result is new to it and requires grad
+        with pytest.raises(RuntimeError, match="constant"):
+            torch.jit.trace(call, first, check_trace=False)
+        return
+    traced = torch.jit.trace(call, first, check_trace=False)
+    other = [2 + t.detach() * 3 for t in leaves()]
+    assert torch.equal(traced(*other), call(*other))

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from engram_rdma_lab_b200 import _native
-from engram_rdma_lab_b200.ops import KeptRows, layer_norm_backward
+from engram_rdma_lab_b200.ops import KeptRows, fp8_weight_grad, layer_norm_backward, layer_norm_forward, restore_fp8, save_fp8
 
 pytestmark = pytest.mark.skipif(not _native.available(), reason="extension not built")
 
@@ -14,3 +14,17 @@ def test_the_second_part_of_a_mean_is_checked(shift):
     x = torch.zeros(4, 256)
     with pytest.raises(ValueError, match="shift must be"):
         layer_norm_backward(x, KeptRows(x, None, torch.zeros(4), torch.ones(4), shift))
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning", "ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("call", [
+    lambda x: layer_norm_forward(x)[0],
+    lambda x: layer_norm_backward(x, KeptRows(x, None, x[:, 0].contiguous(), x[:, 0].contiguous()))[0],
+    lambda x: save_fp8(x)[1],
+    lambda x: restore_fp8(x.to(torch.float8_e4m3fn), torch.ones(4, 2)),
+    lambda x: fp8_weight_grad(x, x.to(torch.float8_e4m3fn), torch.ones(4, 2))[0],
+])
+def test_a_trace_is_refused(call):
+    """A trace would not see the call and keep its result as a constant."""
+    with pytest.raises(RuntimeError, match="constant"):
+        torch.jit.trace(call, (torch.zeros(4, 256),), check_trace=False)
