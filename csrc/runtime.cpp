@@ -490,6 +490,10 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
                                  : index_pointer(indices);
         tokens_ = uint32_t(indices.size(1));
         const uint32_t rows = tokens_ * ept_;
+        // Earlier results lie in the memory that this fetch writes.
+        if (rows > 0)
+            for (c10::VariableVersion &version : output_versions_)
+                version.bump();
         uint32_t ts, hs, ls;
         sf_strides(tokens_, col_major, &ts, &hs, &ls);
         if (rows > 0) {
@@ -1267,20 +1271,32 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
     // PCIe reads at the envelope (50.2 of 51.2 GB/s measured; 8 CTAs: 38).
     int serve_ctas() const { return egm_ ? num_sms_ : 16; }
 
+    // All results of one layer count their changes together, so that autograd
+    // notices when a fetch has overwritten what a backward pass was to read
+    // (inference tensors count none).
+    void share_version(const torch::Tensor &t, uint32_t which) {
+        if (!t.is_inference())
+            t.unsafeGetTensorImpl()->set_version_counter(output_versions_[which]);
+    }
+
     py::list make_outputs(uint32_t ts, uint32_t hs, uint32_t sf_layer_stride) {
         py::list out;
         auto keep = shared_from_this();
         const auto dtype = packs_ ? torch::kFloat8_e4m3fn : torch::kBFloat16;
         auto opts = torch::TensorOptions().dtype(dtype).device(torch::Device(torch::kCUDA, device_));
         auto fopts = torch::TensorOptions().dtype(torch::kFloat32).device(torch::Device(torch::kCUDA, device_));
+        while (output_versions_.size() < 2 * layers_)
+            output_versions_.emplace_back(0);
         const uint64_t arena = arena_->ptr();
         for (uint32_t l = 0; l < layers_; ++l) {
             void *ptr = reinterpret_cast<void *>(arena + dev_output_ + uint64_t(l) * capacity_ * row_bytes_);
             auto data = torch::from_blob(ptr, {int64_t(tokens_), int64_t(hidden_) * ept_}, [keep](void *) {}, opts);
+            share_version(data, 2 * l);
             if (packs_) {
                 void *sptr = reinterpret_cast<void *>(arena + dev_sf_output_ + uint64_t(l) * sf_layer_stride * 4);
                 auto scales = torch::from_blob(sptr, {int64_t(tokens_), int64_t(ept_) * packs_},
                                                {int64_t(ts), int64_t(hs)}, [keep](void *) {}, fopts);
+                share_version(scales, 2 * l + 1);
                 out.append(py::make_tuple(data, scales));
             } else {
                 out.append(data);
@@ -1432,6 +1448,7 @@ class Runtime : public std::enable_shared_from_this<Runtime> {
     std::vector<cudaStream_t> finished_stream_;  // stream of the last eager hook per layer
     // Output views of the last (tokens, scale layout); rebuilt when either changes.
     py::list cached_outputs_;
+    std::vector<c10::VariableVersion> output_versions_;  // [layers][data, scales]
     uint32_t cached_tokens_ = 0xFFFFFFFFu;
     bool cached_col_major_ = true;
     cudaStream_t issue_stream_ = nullptr, owner_stream_ = nullptr;

@@ -420,6 +420,10 @@ class EngramBuffer(EngramBufferBase):
         ``num_qps`` selects how many push channels host-route owners may use
         (0 = all allocated).  ``use_tma_aligned_col_major_sf`` selects the
         column-major, 4-aligned scale layout (default) or row-major.
+
+        Results lie in the buffer's own memory, which the next fetch writes; to
+        autograd that is a change in place, so a backward pass that saved an
+        earlier result raises.
         """
         self._check_fetch_args(indices, self.device, require_cuda=True, allow_pinned=True)
         qps = num_qps or self.num_allocated_qps

@@ -127,7 +127,9 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hid
     """Differentiable layer norm of ``x [tokens, width]``; the arguments are :func:`layer_norm_forward`'s.
 
     ``keep`` (``"fp8"`` or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
-    is wanted.  There is no forward-mode derivative (a tangent raises).  Looked-up e4m3 codes get no gradient
+    is wanted.  ``"exact"`` keeps ``x`` itself: rows that ``EngramBuffer.fetch`` returned last until the next fetch,
+    after which the backward pass raises (not after the replay of a captured fetch, which nothing counts), so take
+    ``"fp8"`` or a copy where fetches run ahead of backward passes.  There is no forward-mode derivative (a tangent raises).  Looked-up e4m3 codes get no gradient
     themselves (:func:`layer_norm_backward` gives their rows').
     """
     if _keep_mode(keep) == 0:
