@@ -29,6 +29,13 @@ __device__ __forceinline__ void keep_mean(const NormForwardParams &p, int64_t r,
     p.shift[r] = (m - (mean - second)) + (shift - second);
 }
 
+// The scale of a block of normalised values.  Where rstd is infinite (a variance
+// that underflowed, and no eps) none of a row's values is finite: scale 1, and
+// 2^-k as NaN makes every code NaN, where the conversion would saturate.
+__device__ __forceinline__ BlockScale kept_scale(float amax, float rstd) {
+    return rstd <= FLT_MAX ? block_scale(amax) : BlockScale{1.f, __uint_as_float(0x7FFFFFFFu)};
+}
+
 // One element of a forward row as fp32.
 template <uint32_t IN> struct RowReader {
     const typename Element<IN>::T *row;
@@ -102,7 +109,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
                 }
             }
             if (p.keep == kKeepFp8) {
-                const BlockScale scale = block_scale(lanes_max(amax));
+                const BlockScale scale = kept_scale(lanes_max(amax), rstd);
                 uint8_t *codes = p.codes + r * p.codes_stride;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -278,7 +285,8 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
             if (there(i)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    // Finite, or NaN in all of a row: an infinity makes the mean NaN or infinite.
+                    // Finite, or in none of a row: an infinity makes the mean NaN or infinite, and rstd
+                    // may be infinite.
                     x[i][e] = mul2(add2(x[i][e], minus_shift), up);
                     if constexpr (FP8)
                         amax = largest3(amax, parts(x[i][e]).x, parts(x[i][e]).y);
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
                 }
             }
             if constexpr (FP8) {
-                const BlockScale unit = block_scale(lanes_max<16>(amax));
+                const BlockScale unit = kept_scale(lanes_max<16>(amax), rstd);
                 if (there(i)) {
                     *reinterpret_cast<uint2 *>(code_at + i * 256) = to_e4m3x8(x[i], unit.down);
                     if (lane % 16 == 0)
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(T0, 1024 / T0)
             for (int q = 0; q < E / 4; ++q) {
                 const float *h = x + q * 4;
                 const BlockScale unit =
-                    block_scale(lanes_max(largest3(largest3(0.f, h[0], h[1]), h[2], h[3])));
+                    kept_scale(lanes_max(largest3(largest3(0.f, h[0], h[1]), h[2], h[3])), rstd);
                 const uint32_t c = c0 - lane + q * kCheckpointBlock;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
