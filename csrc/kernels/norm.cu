@@ -29,9 +29,16 @@ __device__ __forceinline__ void keep_mean(const NormForwardParams &p, int64_t r,
     p.shift[r] = (m - (mean - second)) + (shift - second);
 }
 
+// 1 / sqrt(variance + eps).  The variance may round to below zero, and is NaN
+// where it and its correction overflow fp32: then rstd is NaN as well (fmaxf
+// would make it that of a row without variance).
+__device__ __forceinline__ float row_rstd(float variance, float eps) {
+    return 1.f / sqrtf((variance < 0.f ? 0.f : variance) + eps);
+}
+
 // The scale of a block of normalised values.  Where rstd is infinite (a variance
-// that underflowed, and no eps) none of a row's values is finite: scale 1, and
-// 2^-k as NaN makes every code NaN, where the conversion would saturate.
+// that underflowed, and no eps) or NaN, none of a row's values is finite: scale
+// 1, and 2^-k as NaN makes every code NaN, where the conversion would saturate.
 __device__ __forceinline__ BlockScale kept_scale(float amax, float rstd) {
     return rstd <= FLT_MAX ? block_scale(amax) : BlockScale{1.f, __uint_as_float(0x7FFFFFFFu)};
 }
@@ -82,7 +89,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_con
         }
         const float2 sums = block_sum2(a, b, s_sum[1]);
         const float shift = sums.x * inv;
-        const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
+        const float rstd = row_rstd(sums.y * inv - shift * shift, p.eps);
         if (threadIdx.x == 0) {
             if (p.keep == kKeepStats)
                 keep_mean(p, r, mean, shift);
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
             }
         const float2 sums = warp_rows ? lanes_sum2(total(a), total(b)) : block_sum2(total(a), total(b), s_sum[1]);
         const float shift = sums.x * inv;
-        const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
+        const float rstd = row_rstd(sums.y * inv - shift * shift, p.eps);
         if (share.leader && p.keep != kKeepNothing) {
             if (p.keep == kKeepStats)
                 keep_mean(p, r, mean, shift);
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(T0, 1024 / T0)
             }
         const float2 sums = warp_rows ? lanes_sum2(a, b) : s_sum[1].sum2(a, b);
         const float shift = sums.x * inv;
-        const float rstd = 1.f / sqrtf(fmaxf(sums.y * inv - shift * shift, 0.f) + p.eps);
+        const float rstd = row_rstd(sums.y * inv - shift * shift, p.eps);
         if (share.leader && p.keep != kKeepNothing) {
             if (p.keep == kKeepStats)
                 keep_mean(p, r, mean, shift);

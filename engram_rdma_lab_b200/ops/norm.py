@@ -8,7 +8,8 @@ with one (``keep="fp8"``; the format of :mod:`.checkpoint`), half of bf16's byte
 the gradient needs, and the same checkpoint serves the projection behind the norm
 (:func:`~.projection.fp8_weight_grad`).
 
-Sums over rows and columns are held in fp32 and joined in a fixed order: equal inputs give equal bits on equal GPUs,
+Sums over rows and columns are held in fp32 (a row whose deviations are past 1.8e19 has an infinite or unknown variance:
+its ``y`` is the bias, or NaN) and joined in a fixed order: equal inputs give equal bits on equal GPUs,
 and a row's ``y`` does not depend on the rows beside it.  Everything runs on the current stream and can be captured
 into CUDA graphs (capture the functional pair, not autograd's backward pass).
 """

@@ -5,7 +5,7 @@ import torch
 
 from engram_rdma_lab_b200.ops import layer_norm_forward, restore_fp8
 
-from .test_gpu_readout import FP32, _gpu, randn  # noqa: F401
+from .test_gpu_readout import FP32, _gpu, params, randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,16 @@ def test_infinite_normalised_values_are_kept_as_nan(n, eps):
     assert torch.equal(kept.scales[1], torch.ones_like(kept.scales[1]))
     for r in (0, 2):
         assert torch.isfinite(y[r]).all() and torch.isfinite(restore_fp8(kept.rows, kept.scales, FP32)[r]).all()
+
+
+@pytest.mark.parametrize("n", [256, 1024, 100, 1001, 20001])
+def test_rows_whose_variance_is_beyond_fp32_give_no_finite_garbage(n):
+    """Squares past 3.4e38: the variance is infinite (rstd 0, y the bias) or, where its correction overflows as well,
+    unknown, and then the row is NaN; it is never computed with rstd = 1 / sqrt(eps)."""
+    x = torch.stack([randn(n, n) * 1e20, 1e30 * (1 + randn(n + 1, n).abs() / 16), randn(n + 2, n)])
+    w, b = params(n, FP32)
+    y, kept = layer_norm_forward(x, w, b, keep="exact")
+    for r in (0, 1):
+        assert y[r].isnan().all() or torch.equal(y[r], b)
+        assert kept.rstd[r].isnan() or kept.rstd[r] == 0
+    assert torch.isfinite(y[2]).all()
