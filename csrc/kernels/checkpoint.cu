@@ -162,10 +162,11 @@ __global__ void __launch_bounds__(kThreads) save_any(const __grid_constant__ Sav
 }
 
 // A finite code's value that its type cannot hold (a block's largest value may
-// have been rounded up past it) becomes the type's largest.
-template <uint32_t TYPE> __device__ __forceinline__ float held(float v) {
+// have been rounded up past it) becomes the type's largest.  An infinite scale,
+// which no save writes, makes infinities and not finite values.
+template <uint32_t TYPE> __device__ __forceinline__ float held(float v, float scale) {
     const float most = Element<TYPE>::kLargest;
-    return isnan(v) ? v : fminf(fmaxf(v, -most), most);
+    return isnan(v) || isinf(scale) ? v : fminf(fmaxf(v, -most), most);
 }
 
 // The way back: 8192 x 12288 to bf16 in 54.8 us, 5.5 TB/s (two thirds of what it
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) restore_chunks(const __grid_constant
                     Pair &f = v[e / 4][e % 4];
                     f = mul2(f, both(scale[j]));
                     if (far)
-                        f = pair(held<TYPE>(parts(f).x), held<TYPE>(parts(f).y));
+                        f = pair(held<TYPE>(parts(f).x, scale[j]), held<TYPE>(parts(f).y, scale[j]));
                 }
                 if constexpr (TYPE == kFp32) {
                     store_row8<TYPE>(x, v[0]);
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) restore_any(const __grid_constant__ 
             for (int i = 0; i < 4; ++i) {
                 const uint32_t c = block[j] * kCheckpointBlock + i * 32 + lane;
                 if (there[j] && c < p.width)
-                    x[c] = Element<TYPE>::put(held<TYPE>(Element<kE4m3>::get(code[j][i]) * scale[j]));
+                    x[c] = Element<TYPE>::put(held<TYPE>(Element<kE4m3>::get(code[j][i]) * scale[j], scale[j]));
             }
         }
     }

@@ -5,7 +5,7 @@ import torch
 
 from engram_rdma_lab_b200.ops import layer_norm_forward, restore_fp8
 
-from .test_gpu_readout import FP32, _gpu, params, randn  # noqa: F401
+from .test_gpu_readout import BF16, F8, FP16, FP32, _gpu, params, randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,18 @@ def test_rows_whose_variance_is_beyond_fp32_give_no_finite_garbage(n):
         assert y[r].isnan().all() or torch.equal(y[r], b)
         assert kept.rstd[r].isnan() or kept.rstd[r] == 0
     assert torch.isfinite(y[2]).all()
+
+
+@pytest.mark.parametrize("n", [256, 1000])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_restore_keeps_infinite_values_infinite(n, dtype):
+    """Scales of another origin may be infinite: their values are infinities (NaN for codes of zero), while finite
+    values past the type's range become its largest."""
+    codes = torch.ones(3, n, device="cuda").to(F8)
+    codes[:, 1], codes[:, 2] = torch.tensor(-2.0).to(F8), torch.tensor(0.0).to(F8)
+    scales = torch.ones(3, -(-n // 128), device="cuda")
+    scales[1, 0], scales[2] = float("inf"), 2.0 ** 127
+    x = restore_fp8(codes, scales, dtype)
+    assert torch.isposinf(x[1, 0]) and torch.isneginf(x[1, 1]) and x[1, 2].isnan() and torch.isinf(x[1, 3:128]).all()
+    assert torch.isfinite(x[0]).all() and torch.isfinite(x[1, 128:]).all() and torch.isfinite(x[2]).all()
+    assert x[2, 1] == (-torch.finfo(dtype).max)
