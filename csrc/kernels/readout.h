@@ -89,13 +89,18 @@ struct WeightGradParams {
     float *dy_sums;                       // [out] fp32 column sums of dy; nullptr: not needed
     float *sum_parts;                     // [sum_rows][out], what dy_sums adds up
     void *dy_planes;                      // [planes][rows][plane_stride] bf16; nullptr: dy itself serves
-    float *dw_parts;                      // [parts][out][width], parts > 1
+    float *dw_parts;                      // [slots][out][width], parts > 1
     uint32_t *fault;                      // host-mapped: set when a wait ran out
     int64_t rows, dy_stride, codes_stride, scale_row_stride, scale_col_stride, plane_stride;
     uint32_t width, out, type, param_type, out_type, sum_rows;
     // The plan (plan_weight_grad): dy as `planes` bf16 terms; pairs of blocks for
-    // `halves` x 256 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64.
+    // `halves` x 256 outputs by tile_k columns; the rows in `parts` of `part_steps` x 64,
+    // each with all terms of its rows.
     uint32_t planes, halves, tile_k, tiles_k, tiles_o, parts, part_steps;
+    // At most `slots` parts at a time; of later launches slot 0 holds the sum of the
+    // parts before.  A launch's parts start at first_part, in first_slot, and its
+    // join adds up `joined` slots, into dweight with the last.
+    uint32_t slots, first_part, first_slot, joined, last;
     uint32_t boxes;  // results leave by tiled stores
 };
 

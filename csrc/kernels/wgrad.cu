@@ -14,7 +14,9 @@
 // rounding it, an error that goes with the accumulator's size and the number of
 // additions: the smallest terms go first, while the accumulator is small (512
 // rows of fp32 are 1.5e-7 of the result's norm off, with the largest term first
-// they were 2.5e-6).
+// they were 2.5e-6), and an accumulator takes a limited number of rows before it is
+// rounded into the sum of its like (most_steps), so that the error does not grow
+// with the rows.
 #include <algorithm>
 
 #include "../driver.h"
@@ -111,6 +113,14 @@ __global__ void __launch_bounds__(kThreads) split_dy(const __grid_constant__ Wei
 
 // ---------------------------------------------------------------- the product
 constexpr uint32_t kSteps = 64;              // rows per stage
+constexpr int64_t kPartBytes = 512 << 20;    // workspace for parts of the rows
+
+// Stages of the rows that one accumulator takes, four additions each.  What the
+// cuts of its additions take grows with their number, 7e-9 of the result's norm
+// for each: 3.7e-6 for 8192 rows.  A 16-bit result loses 1.7e-3 to its rounding
+// anyway; an fp32 one goes by 2048 rows, 6.5e-7 whatever their number (8192 x
+// 12288 to 2048: bf16 dy 512 us, 289 in one accumulator; fp32 dy 1014 us).
+__host__ __device__ constexpr uint32_t most_steps(uint32_t out_type) { return out_type == kFp32 ? 32 : 128; }
 constexpr int kLoadStages = 4, kOperandStages = 3;
 constexpr uint32_t kDyChunk = kSteps * 128;  // 64 columns of dy (bf16)
 constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
@@ -195,7 +205,7 @@ __device__ __forceinline__ void store_shared16(uint32_t at, const Vec16 &v) {
 // stores where rows are on 16-byte boundaries, else row by row.
 template <uint32_t TYPE>
 __device__ __forceinline__ void store_tile(const WeightGradParams &p, const CUtensorMap *map, const Shared &s, uint32_t tmem,
-                                           uint8_t *boxes, uint32_t o0, uint32_t k0, uint32_t part) {
+                                           uint8_t *boxes, uint32_t o0, uint32_t k0, uint32_t slot) {
     constexpr uint32_t kSize = element_bytes(TYPE), kRow = 32 * kSize;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, columns = min(p.tile_k, p.width - k0);
     const uint32_t half = p.halves == 2 ? warp / 4 : 0, row0 = warp % 4 * 32;
@@ -252,7 +262,7 @@ __device__ __forceinline__ void store_tile(const WeightGradParams &p, const CUte
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                tensor_store_3d(map, int(k0 + c0), int(o_first), int(part), at);
+                tensor_store_3d(map, int(k0 + c0), int(o_first), int(slot), at);
                 bulk_commit();
             }
             box = box + 1 == kBoxes ? 0 : box + 1;
@@ -260,7 +270,7 @@ __device__ __forceinline__ void store_tile(const WeightGradParams &p, const CUte
             __syncwarp();
             using T = typename Element<TYPE>::T;
             T *out = p.parts == 1 ? static_cast<T *>(p.dweight)
-                                  : reinterpret_cast<T *>(p.dw_parts + int64_t(part) * p.out * p.width);
+                                  : reinterpret_cast<T *>(p.dw_parts + int64_t(slot) * p.out * p.width);
             const uint32_t o_rows = min(32u, p.out - o_first), chunk = lane * kSize / 16;
             if (c0 + lane < columns)
 #pragma unroll 8
@@ -308,10 +318,11 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     const uint32_t o0 = tile % p.tiles_o * (p.halves * 256) + rank * 128;  // half h: o0 + h * 256
     const uint32_t tile_k0 = tile / p.tiles_o % p.tiles_k * p.tile_k;
     const uint32_t k0 = tile_k0 + rank * share;                            // this block's columns to decode
-    const uint32_t part = tile / (p.tiles_o * p.tiles_k);
+    const uint32_t place = tile / (p.tiles_o * p.tiles_k), part = p.first_part + place, slot = p.first_slot + place;
     const uint32_t plane_steps = uint32_t((p.rows + kSteps - 1) / kSteps);
-    const uint32_t first = part * p.part_steps;
-    const uint32_t steps = min(p.part_steps, plane_steps * p.planes - first);
+    // A part's rows, once for each term of dy, the smallest term first.
+    const uint32_t first = part * p.part_steps, row_steps = min(p.part_steps, plane_steps - first);
+    const uint32_t steps = row_steps * p.planes;
     const uint32_t columns = k0 < p.width ? min(share, p.width - k0) : 0;
 
     if (threadIdx.x == 0) {
@@ -346,11 +357,11 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
             const uint32_t code_chunks = (columns + 63) / 64;
             uint32_t i = 0;
             for (; ok && i < steps; ++i) {
-                const uint32_t at = i % kLoadStages, g = first + i;
+                const uint32_t at = i % kLoadStages;
                 ok = mbar_wait_often(&s.load_free[at], (i / kLoadStages & 1) ^ 1, kWaitNs);
                 if (!ok)
                     break;
-                const int m = int(g % plane_steps * kSteps), plane = int(p.planes - 1 - g / plane_steps);
+                const int m = int((first + i % row_steps) * kSteps), plane = int(p.planes - 1 - i / row_steps);
                 mbar_arrive_expect_tx(&s.loaded[at], dy_chunks * kDyChunk + code_chunks * kCodeChunk);
                 for (uint32_t c = 0; c < dy_chunks; ++c)
                     tensor_load_3d(dy_tiles + at * kDyBytes + c * kDyChunk, &dy_map, int(o0 + c / 2 * 256 + c % 2 * 64), m,
@@ -397,7 +408,7 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
         const float *scales = p.scales + block0 * p.scale_col_stride;
         float next[kAhead][2][kBlocks];
         auto load = [&](uint32_t i, float (&to)[2][kBlocks]) {
-            const int64_t m = int64_t((first + i) % plane_steps) * kSteps + lane;
+            const int64_t m = int64_t(first + i % row_steps) * kSteps + lane;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
@@ -540,11 +551,11 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
             uint8_t *boxes = ring + warp * (kBoxes * kBoxBytes);
             const uint32_t type = p.parts == 1 ? p.out_type : uint32_t(kFp32);
             if (type == kBf16)
-                store_tile<kBf16>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+                store_tile<kBf16>(p, &out_map, s, tmem, boxes, o0, tile_k0, slot);
             else if (type == kFp16)
-                store_tile<kFp16>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+                store_tile<kFp16>(p, &out_map, s, tmem, boxes, o0, tile_k0, slot);
             else
-                store_tile<kFp32>(p, &out_map, s, tmem, boxes, o0, tile_k0, part);
+                store_tile<kFp32>(p, &out_map, s, tmem, boxes, o0, tile_k0, slot);
         }
         tensor_fence_before();
         if (!ok && lane == 0)
@@ -560,13 +571,17 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     }
 }
 
-// Adds the parts of the rows in order, and folds the norm in.
+// Adds the parts of the rows in order, and folds the norm in with the last.
 __global__ void __launch_bounds__(kThreads) weight_grad_join(const __grid_constant__ WeightGradParams p) {
     const int64_t total = int64_t(p.out) * p.width, stride = int64_t(gridDim.x) * kThreads;
     for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total; at += stride) {
         float v = 0.f;
-        for (uint32_t part = 0; part < p.parts; ++part)
-            v += p.dw_parts[part * total + at];
+        for (uint32_t slot = 0; slot < p.joined; ++slot)
+            v += p.dw_parts[slot * total + at];
+        if (!p.last) {
+            p.dw_parts[at] = v;
+            continue;
+        }
         const int64_t o = at / p.width;
         const uint32_t k = uint32_t(at - o * p.width);
         if (p.norm_weight != nullptr)
@@ -617,20 +632,22 @@ void plan_weight_grad(WeightGradParams &p, int num_sms) {
     p.planes = p.type == kBf16 ? 1 : p.type == kFp16 ? 2 : 3;
     p.halves = p.out > 256 ? 2 : 1;
     p.tiles_o = (p.out + p.halves * 256 - 1) / (p.halves * 256);
-    const int64_t steps = (p.rows + kSteps - 1) / kSteps * p.planes, pairs = num_sms / 2;
+    const int64_t steps = (p.rows + kSteps - 1) / kSteps, pairs = num_sms / 2;
     // Cycles of one pair: a stage is bound by its MMAs (256 x 16 x n takes n / 2)
     // or by shared memory (128 bytes a cycle: dy in and out, codes in and out,
     // operands in, and out for each half); the epilogue moves ~12 values a cycle
     // and block.  Splitting the rows costs a pass over the parts at ~3.5 KB a cycle.
     double best = 1e300;
+    const int64_t limit = most_steps(p.out_type), fewest = (steps + limit - 1) / limit;
+    const int64_t most = std::max(fewest, std::min<int64_t>(steps, 64));
     for (uint32_t tile = 32; tile <= 256; tile += 32) {
         const uint32_t tiles_k = (p.width + tile - 1) / tile;
         const int64_t tiles = int64_t(p.tiles_o) * tiles_k;
-        for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 64); parts = parts < 8 ? parts + 1 : parts * 2) {
+        for (int64_t parts = fewest; parts <= most; parts = parts < 8 ? parts + 1 : parts * 2) {
             const int64_t part_steps = (steps + parts - 1) / parts, used = (steps + part_steps - 1) / part_steps;
             const double waves = double((tiles * used + pairs - 1) / pairs);
             const double stage = std::max({2.0 * p.halves * tile, 256.0 * p.halves + (1 + p.halves / 2.) * tile, 400.});
-            const double block = 5000 + part_steps * stage + p.halves * 128.0 * tile / 12;
+            const double block = 5000 + part_steps * p.planes * stage + p.halves * 128.0 * tile / 12;
             const double join = used > 1 ? 3000 + 8.0 * used * p.out * p.width / 3500 : 0;
             const double cost = waves * block + join;
             if (cost < best * 0.999) {
@@ -642,6 +659,8 @@ void plan_weight_grad(WeightGradParams &p, int num_sms) {
             }
         }
     }
+    const int64_t room = kPartBytes / (4 * int64_t(p.out) * p.width);
+    p.slots = uint32_t(std::min<int64_t>(p.parts, std::max<int64_t>(2, room)));
 }
 
 cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
@@ -665,23 +684,31 @@ cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
         out_map = tile_map(type == kBf16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                            : type == kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                           p.parts == 1 ? p.dweight : p.dw_parts, p.width, p.out, p.parts,
+                           p.parts == 1 ? p.dweight : p.dw_parts, p.width, p.out, p.slots,
                            uint64_t(p.width) * element_bytes(type), 32, 32,
                            type == kFp32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     cudaError_t rc = cudaFuncSetAttribute(weight_grad_tensor, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
     if (rc != cudaSuccess)
         return rc;
-    const dim3 grid(2 * p.tiles_o * p.tiles_k * p.parts);
-    if (p.dy_sums != nullptr) {
-        rc = launch_overlapped(weight_grad_tensor, grid, kTensorThreads, kSharedBytes, stream, q, dy_map, code_map, out_map);
-        if (rc != cudaSuccess)
-            return rc;
-    } else {
-        weight_grad_tensor<<<grid, kTensorThreads, kSharedBytes, stream>>>(q, dy_map, code_map, out_map);
-    }
-    if (p.parts > 1) {
-        const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
-        weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(p);
+    for (uint32_t first = 0; first < p.parts;) {
+        q.first_part = first;
+        q.first_slot = first == 0 ? 0 : 1;
+        const uint32_t count = std::min(p.parts - first, p.slots - q.first_slot);
+        const dim3 grid(2 * p.tiles_o * p.tiles_k * count);
+        if (first == 0 && p.dy_sums != nullptr) {
+            rc = launch_overlapped(weight_grad_tensor, grid, kTensorThreads, kSharedBytes, stream, q, dy_map, code_map, out_map);
+            if (rc != cudaSuccess)
+                return rc;
+        } else {
+            weight_grad_tensor<<<grid, kTensorThreads, kSharedBytes, stream>>>(q, dy_map, code_map, out_map);
+        }
+        first += count;
+        q.joined = q.first_slot + count;
+        q.last = first == p.parts;
+        if (p.parts > 1) {
+            const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
+            weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(q);
+        }
     }
     return cudaGetLastError();
 }

@@ -418,7 +418,7 @@ py::tuple fp8_weight_grad(const Tensor &dy, const Tensor &codes, const Tensor &s
         p.dy_planes = planes->data_ptr();
     }
     if (p.parts > 1) {
-        dw_parts = empty({int64_t(p.parts), out, width}, ScalarType::Float, dy);
+        dw_parts = empty({int64_t(p.slots), out, width}, ScalarType::Float, dy);
         p.dw_parts = static_cast<float *>(dw_parts->data_ptr());
     }
     check_cuda(launch_weight_grad(p, at::cuda::getCurrentCUDAStream(device).stream()), "launch weight gradient");

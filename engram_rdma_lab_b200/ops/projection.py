@@ -24,8 +24,9 @@ def fp8_weight_grad(dy, codes, scales, norm_weight=None, norm_bias=None, *, dtyp
     ``"fp8"``; with ``norm_weight`` (and ``norm_bias``), ``[width]`` of dy's type or fp32, the projection's input was
     ``X * norm_weight + norm_bias``.  Both results have dy's type, or ``dtype`` fp32; ``dbias`` is None without
     ``bias_grad``.  Products are exact (dy enters as bf16 terms that hold all of its bits, the checkpoint's values are
-    exact in bf16; scales that are no powers of two round them to bf16) and summed in fp32 on the tensor cores: 2048
-    rows of fp32 are about 4e-7 of the result's norm off.
+    exact in bf16; scales that are no powers of two round them to bf16) and summed in fp32 on the tensor cores, which
+    cut what they add.  An fp32 result takes 2048 rows into one sum and joins those by rounded additions: it is 7e-7 of
+    its norm off, whatever the number of rows.  A 16-bit result takes 8192 rows into one sum, 4e-6 beside its rounding.
     """
     return _native.load().fp8_weight_grad(dy, codes, scales, norm_weight, norm_bias, dtype, bias_grad)
 
