@@ -10,6 +10,8 @@ with ``n = h w + b``, ``dW = dz^T n = (dz^T h) w + (sum dz) b^T``.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -31,6 +33,17 @@ def fp8_weight_grad(dy, codes, scales, norm_weight=None, norm_bias=None, *, dtyp
     return _native.load().fp8_weight_grad(dy, codes, scales, norm_weight, norm_bias, dtype, bias_grad)
 
 
+def _backward_as_written(backward):
+    """A projection's backward pass: its products in the parameters' type, also where it runs under autocast."""
+
+    @functools.wraps(backward)
+    def run(ctx, dz):
+        with torch.autocast(dz.device.type, enabled=False):
+            return backward(ctx, dz)
+
+    return once_differentiable(run)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -40,7 +53,7 @@ class _Linear(torch.autograd.Function):
         return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
-    @once_differentiable
+    @_backward_as_written
     def backward(ctx, dz):
         codes, scales, weight = ctx.saved_tensors
         dz = _adjacent(dz).to(weight.dtype)  # autocast may have changed the product's type
@@ -69,7 +82,7 @@ class _NormLinear(torch.autograd.Function):
         return torch.nn.functional.linear(normed, weight, bias)
 
     @staticmethod
-    @once_differentiable
+    @_backward_as_written
     def backward(ctx, dz):
         codes, scales, rstd, norm_weight, norm_bias, weight = ctx.saved_tensors
         need = ctx.needs_input_grad

@@ -10,6 +10,7 @@ import threading
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+import torch.utils.checkpoint
 
 from engram_rdma_lab_b200 import _native, ops
 
@@ -150,3 +151,34 @@ def test_a_trace_computes_with_its_own_inputs(form, grad):
     traced = torch.jit.trace(call, first, check_trace=False)
     other = [2 + t.detach() * 3 for t in leaves()]
     assert torch.equal(traced(*other), call(*other))
+
+
+# ---------------------------------------------------------------- autocast
+@pytest.mark.parametrize("dtype,other", [(FP32, BF16), (BF16, FP16), (FP16, BF16)])
+@pytest.mark.parametrize("form", ["linear", "norm_linear"])
+def test_gradients_do_not_depend_on_where_backward_runs(form, dtype, other):
+    """A backward pass inside the region computes what it does outside: products in the parameters' type."""
+    def gradients(inside):
+        x, nw, nb, w, b = (t.requires_grad_() for t in leaves(dtype))
+        used = (x, w, b) if form == "linear" else (x, nw, nb, w, b)
+        with torch.autocast("cpu", other):
+            z = ops.linear(x, w, b) if form == "linear" else ops.norm_linear(x, nw, nb, w, b)
+            assert z.dtype == other
+            if inside:
+                return torch.autograd.grad(z, used, randn(9, *z.shape, dtype=other))
+        return torch.autograd.grad(z, used, randn(9, *z.shape, dtype=other))
+
+    for a, c in zip(gradients(True), gradients(False)):
+        assert a.dtype == c.dtype == dtype and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("form", [*FORMS, "linear"])
+def test_recomputed_under_activation_checkpointing(form):
+    call = FORMS[form][0] if form in FORMS else lambda x, nw, nb, w, b: ops.linear(x, w, b)
+    results = []
+    for recompute in (False, True):
+        values = [t.requires_grad_() for t in leaves()]
+        z = torch.utils.checkpoint.checkpoint(call, *values, use_reentrant=False) if recompute else call(*values)
+        z.backward(randn(9, *z.shape))
+        results.append([t.grad for t in values])
+    assert all(a is b is None or torch.equal(a, b) for a, b in zip(*results))
