@@ -16,7 +16,9 @@ from ..ops import norm_linear
 class EngramReadout(torch.nn.Module):
     """``layer_norm(rows) @ weight^T + bias`` for rows of ``entries`` looked-up rows of ``hidden`` columns each.
 
-    ``block`` is the columns per scale of e4m3 tables.  Parameters have ``dtype``, and so has the result.
+    ``block`` is the columns per scale of e4m3 tables.  Parameters have ``dtype``, and so has the result (autocast's
+    type under autocast): rows of that type, e4m3 codes with their scales or, with fp32 parameters, bf16 and fp16 rows,
+    which are widened first (exactly, and not kept).
     """
 
     def __init__(self, hidden: int, entries: int, features: int, *, bias: bool = False, eps: float = 1e-5,
@@ -35,4 +37,6 @@ class EngramReadout(torch.nn.Module):
     def forward(self, data: torch.Tensor, scales: torch.Tensor | None = None) -> torch.Tensor:
         lookup = {} if scales is None else dict(scales=scales, hidden=self.hidden, block=self.block,
                                                 dtype=self.weight.dtype)
+        if scales is None and self.weight.dtype == torch.float32 and data.dtype in (torch.bfloat16, torch.float16):
+            data = data.float()
         return norm_linear(data, self.norm_weight, self.norm_bias, self.weight, self.bias, self.eps, **lookup)

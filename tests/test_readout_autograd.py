@@ -13,6 +13,7 @@ import torch.autograd.forward_ad as forward_ad
 import torch.utils.checkpoint
 
 from engram_rdma_lab_b200 import _native, ops
+from engram_rdma_lab_b200.models import EngramReadout
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -182,3 +183,30 @@ def test_recomputed_under_activation_checkpointing(form):
         z.backward(randn(9, *z.shape))
         results.append([t.grad for t in values])
     assert all(a is b is None or torch.equal(a, b) for a, b in zip(*results))
+
+
+# ---------------------------------------------------------------- the module
+@pytest.mark.parametrize("rows", [BF16, FP16, FP32])
+def test_a_readout_with_fp32_parameters_takes_16_bit_rows(rows):
+    """The rows' values are exact in fp32: parameters and result have the module's type."""
+    torch.manual_seed(1)
+    readout = EngramReadout(64, 4, 24, bias=True, dtype=FP32)
+    x = randn(1, 10, 256, dtype=rows).requires_grad_()
+    z = readout(x)
+    parameters = list(readout.parameters())
+    want = ops.norm_linear(x.detach().float(), *parameters[:4])
+    assert z.dtype == FP32 and torch.equal(z, want)
+    dz = randn(2, *z.shape)
+    got = torch.autograd.grad(z, [x, *parameters], dz)
+    assert got[0].dtype == rows and all(torch.equal(a, c) for a, c in zip(got[1:], torch.autograd.grad(want, parameters, dz)))
+    with torch.autocast("cpu", BF16):
+        assert readout(x).dtype == BF16
+
+
+def test_a_readout_refuses_rows_that_its_type_cannot_hold():
+    with pytest.raises(ValueError, match="rows' type"):
+        EngramReadout(64, 4, 24, dtype=FP16)(randn(1, 10, 256, dtype=BF16))
+    with pytest.raises(ValueError, match="rows' type"):
+        EngramReadout(64, 4, 24, dtype=BF16)(randn(1, 10, 256))
+    with pytest.raises(ValueError):
+        EngramReadout(64, 4, 24, dtype=FP32)(randn(1, 10, 256).to(torch.float8_e4m3fn))
