@@ -142,7 +142,7 @@ uint32_t *fault_word(int device) {
 }
 
 // The word, read before every launch without synchronising: a set one refuses
-// all further launches.
+// all further calls.  Replays of captured calls do not come here (check_readout).
 uint32_t *healthy_word(int device) {
     uint32_t *word = fault_word(device);
     check(*static_cast<const volatile uint32_t *>(word) == 0,
@@ -313,6 +313,7 @@ py::tuple save_fp8(const Tensor &x, bool recorded) {
     const int64_t rows = x.size(0), width = x.size(1);
     const Tensor codes = empty_codes(x, rows, width), scales = empty_scales(x, rows, width);
     if (rows > 0) {
+        healthy_word(device);
         SaveFp8Params p{};
         p.x = x.data_ptr();
         p.codes = static_cast<uint8_t *>(codes.data_ptr());
@@ -338,6 +339,7 @@ Tensor restore_fp8(const Tensor &codes, const Tensor &scales, ScalarType dtype) 
     const int64_t rows = codes.size(0), width = codes.size(1);
     const Tensor x = empty({rows, width}, dtype, codes);
     if (rows > 0) {
+        healthy_word(device);
         RestoreFp8Params p{};
         p.codes = static_cast<const uint8_t *>(codes.data_ptr());
         p.scales = static_cast<const float *>(scales.data_ptr());
@@ -433,6 +435,9 @@ void bind_readout(py::module_ &m) {
           py::arg("recorded") = false);
     m.def("norm_backward", &norm_backward, py::arg("dy"), py::arg("kept"), py::arg("scales"), py::arg("mean"),
           py::arg("rstd"), py::arg("weight"), py::arg("want_dx"), py::arg("want_params"), py::arg("shift"));
+    m.def(
+        "check_readout", [](int device) { healthy_word(device); }, py::arg("device"),
+        "Raise if a read-out kernel on this GPU gave up waiting.");
     m.def(
         "debug_readout_fault",
         [](int device, uint32_t code) { return std::exchange(*static_cast<volatile uint32_t *>(fault_word(device)), code); },

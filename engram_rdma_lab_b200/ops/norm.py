@@ -11,7 +11,8 @@ the gradient needs, and the same checkpoint serves the projection behind the nor
 Sums over rows and columns are held in fp32 (a row whose deviations are past 1.8e19 has an infinite or unknown variance:
 its ``y`` is the bias, or NaN) and joined in a fixed order: equal inputs give equal bits on equal GPUs,
 and a row's ``y`` does not depend on the rows beside it.  Everything runs on the current stream and can be captured
-into CUDA graphs (capture the functional pair, not autograd's backward pass).
+into CUDA graphs (capture the functional pair, not autograd's backward pass).  A kernel whose bounded wait for its
+own copies ran out reports that: the read-out calls that follow raise, and :func:`check_readout` asks.
 """
 
 from __future__ import annotations
@@ -80,6 +81,20 @@ def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True
     """
     return _native.load().norm_backward(dy, kept.rows, kept.scales, kept.mean, kept.rstd, weight, want_dx, want_params,
                                         kept.shift)
+
+
+def check_readout(device=None) -> None:
+    """Wait for the device (default: the current one) and raise if a read-out kernel gave up waiting on it.
+
+    Every read-out call raises then too, but it looks when it is made: replays of captured calls report nothing, nor do
+    the last calls before their results are used.  Results computed before this returns are good.
+    """
+    device = torch.device("cuda" if device is None else f"cuda:{device}" if isinstance(device, int) else device)
+    if device.type != "cuda":
+        raise ValueError("read-out kernels run on GPUs")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    torch.cuda.synchronize(index)
+    _native.load().check_readout(index)
 
 
 def _adjacent(t: torch.Tensor) -> torch.Tensor:

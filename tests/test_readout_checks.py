@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from engram_rdma_lab_b200 import _native
-from engram_rdma_lab_b200.ops import KeptRows, fp8_weight_grad, layer_norm_backward, layer_norm_forward, restore_fp8, save_fp8
+from engram_rdma_lab_b200.ops import KeptRows, check_readout, fp8_weight_grad, layer_norm_backward, layer_norm_forward, restore_fp8, save_fp8
 
 pytestmark = pytest.mark.skipif(not _native.available(), reason="extension not built")
 
@@ -28,3 +28,8 @@ def test_a_trace_is_refused(call):
     """A trace would not see the call and keep its result as a constant."""
     with pytest.raises(RuntimeError, match="constant"):
         torch.jit.trace(call, (torch.zeros(4, 256),), check_trace=False)
+
+
+def test_a_check_of_another_kind_of_device():
+    with pytest.raises(ValueError, match="on GPUs"):
+        check_readout("cpu")
