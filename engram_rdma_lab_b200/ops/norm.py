@@ -28,18 +28,26 @@ from .. import _native
 _KEEP = {None: 0, "exact": 1, "fp8": 2}
 
 
-class KeptRows(NamedTuple):
-    """What ``layer_norm_forward`` keeps: ``(x, None, mean, rstd, shift)`` or ``(codes, scales, None, rstd)``.
-
-    A row's mean is ``mean + shift``: the rounded mean, and what its rounding left (None: zeros), which counts where a
-    row's offset is many times its deviation.
-    """
-
+class _KeptRows(NamedTuple):
     rows: torch.Tensor
     scales: Optional[torch.Tensor]
     mean: Optional[torch.Tensor]
     rstd: torch.Tensor
+
+
+class KeptRows(_KeptRows):
+    """What ``layer_norm_forward`` keeps: ``(x, None, mean, rstd)`` or ``(codes, scales, None, rstd)``.
+
+    Beside the four, ``shift`` is what the rounding of ``mean`` left (None: zeros): a row's mean is ``mean + shift``,
+    which counts where its offset is many times its deviation.
+    """
+
     shift: Optional[torch.Tensor] = None
+
+    def __new__(cls, rows, scales, mean, rstd, shift=None):
+        self = super().__new__(cls, rows, scales, mean, rstd)
+        self.shift = shift
+        return self
 
 
 def _keep_mode(keep) -> int:
@@ -125,7 +133,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, scales, hidden, block, dtype, keep):
         y, kept = _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, True)
-        ctx.save_for_backward(*kept, weight)
+        ctx.save_for_backward(*kept, kept.shift, weight)
         return y
 
     @staticmethod

@@ -1,5 +1,8 @@
 """Argument checks of the read-out operators beyond test_readout_refusals.py (no GPU is touched)."""
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -33,3 +36,13 @@ def test_a_trace_is_refused(call):
 def test_a_check_of_another_kind_of_device():
     with pytest.raises(ValueError, match="on GPUs"):
         check_readout("cpu")
+
+
+def test_kept_rows_are_four_and_carry_the_rest_of_the_mean():
+    """They unpack as (rows, scales, mean, rstd); copies have what is beside the four, a tuple of the four has none."""
+    kept = KeptRows(torch.ones(4, 8), None, torch.zeros(4), torch.ones(4), torch.full((4,), 2.0))
+    rows, scales, mean, rstd = kept
+    assert rows is kept.rows and scales is None and mean is kept.mean and rstd is kept.rstd
+    for same in (copy.copy(kept), copy.deepcopy(kept), pickle.loads(pickle.dumps(kept))):
+        assert torch.equal(same.shift, kept.shift) and torch.equal(same.rows, rows) and len(same) == 4
+    assert KeptRows(*kept).shift is None and kept._replace(rstd=mean).shift is None
