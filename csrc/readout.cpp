@@ -99,6 +99,14 @@ Tensor empty(at::IntArrayRef size, ScalarType dtype, const Tensor &like) {
     return at::detail::empty_cuda(size, dtype, like.device(), std::nullopt);
 }
 
+// Row `at` of a new tensor [.., width] as a tensor of its own.
+Tensor row_of(const Tensor &all, int64_t at) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    impl->set_storage_offset(at * all.size(1));
+    impl->set_sizes_contiguous({all.size(1)});
+    return Tensor(std::move(impl));
+}
+
 // Code rows start on 16-byte boundaries, so every kernel can read them in vectors.
 Tensor empty_codes(const Tensor &like, int64_t rows, int64_t width) {
     return at::detail::empty_strided_cuda({rows, width}, {(width + 15) / 16 * 16, 1}, ScalarType::Float8_e4m3fn,
@@ -188,13 +196,15 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
     c10::cuda::CUDAGuard guard(device);
     const Tensor y = empty({rows, width}, out, x);
     OptTensor codes, code_scales, mean, rstd, shift;
-    if (keep != kKeepNothing)
-        rstd = empty({rows}, ScalarType::Float, x);
     if (keep == kKeepStats) {
-        mean = empty({rows}, ScalarType::Float, x);
-        shift = empty({rows}, ScalarType::Float, x);
+        // One allocation for the three (each takes as long as a check of all arguments).
+        const Tensor stats = empty({3, rows}, ScalarType::Float, x);
+        mean = row_of(stats, 0);
+        shift = row_of(stats, 1);
+        rstd = row_of(stats, 2);
     }
     if (keep == kKeepFp8) {
+        rstd = empty({rows}, ScalarType::Float, x);
         codes = empty_codes(x, rows, width);
         code_scales = empty_scales(x, rows, width);
     }

@@ -45,8 +45,9 @@ class KeptRows(_KeptRows):
     shift: Optional[torch.Tensor] = None
 
     def __new__(cls, rows, scales, mean, rstd, shift=None):
-        self = super().__new__(cls, rows, scales, mean, rstd)
-        self.shift = shift
+        self = tuple.__new__(cls, (rows, scales, mean, rstd))
+        if shift is not None:
+            self.shift = shift
         return self
 
 
@@ -63,7 +64,9 @@ def _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, recorded)
         x, weight, bias, eps, scales, hidden, block, dtype, mode, recorded)
     if mode == 0:
         return y, None
-    return y, KeptRows(x, None, mean, rstd, shift) if mode == 1 else KeptRows(codes, code_scales, None, rstd)
+    if mode == 2:
+        return y, KeptRows(codes, code_scales, None, rstd)
+    return y, KeptRows(x, None, mean, rstd, shift)
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hidden=None, block: int = 128,
