@@ -82,8 +82,29 @@ void need_checkpoint(const Tensor &codes, const Tensor &scales) {
          "scales must be float32 [rows, ceil(width / 128)]");
 }
 
+// A tensor whose values lie in memory of its own, all of it there.  Fake and
+// functionalised tensors, masked ones and freed storages (a sharded parameter's
+// between its uses) have null pointers; a negated view's values are not what lies
+// in its memory.
+void need_plain(const Tensor &t) {
+    need(t.layout() == at::kStrided && t.has_storage() && !t.is_neg() && !t._is_zerotensor(),
+         "tensors must be plain, with their values in memory");
+    if (t.numel() == 0)
+        return;
+    int64_t last = t.storage_offset();
+    for (int64_t d = 0; d < t.dim(); ++d)
+        last += (t.size(d) - 1) * t.stride(d);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    need(size_t(last + 1) * t.element_size() <= t.storage().nbytes() && at != 0 && at % t.element_size() == 0,
+         "tensors must be plain, with their values in memory");
+}
+
 // The device all of these are on, which has to be a GPU.
 int need_device(const Tensor &first, std::initializer_list<const OptTensor *> others) {
+    need_plain(first);
+    for (const OptTensor *t : others)
+        if (*t)
+            need_plain(**t);
     need(first.is_cuda(), "tensors must be on a GPU");
     for (const OptTensor *t : others)
         need(!*t || (*t)->device() == first.device(), "tensors must be on one GPU");

@@ -5,6 +5,8 @@ import pickle
 
 import pytest
 import torch
+import torch.masked
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from engram_rdma_lab_b200 import _native
 from engram_rdma_lab_b200.ops import KeptRows, check_readout, fp8_weight_grad, layer_norm_backward, layer_norm_forward, restore_fp8, save_fp8
@@ -46,3 +48,85 @@ def test_kept_rows_are_four_and_carry_the_rest_of_the_mean():
     for same in (copy.copy(kept), copy.deepcopy(kept), pickle.loads(pickle.dumps(kept))):
         assert torch.equal(same.shift, kept.shift) and torch.equal(same.rows, rows) and len(same) == 4
     assert KeptRows(*kept).shift is None and kept._replace(rstd=mean).shift is None
+
+
+# ---------------------------------------------------------------- tensors without memory
+def masked(t):
+    return torch.masked.masked_tensor(t, torch.ones_like(t, dtype=torch.bool))
+
+
+def freed(t):
+    t = t.clone()
+    t.untyped_storage().resize_(0)
+    return t
+
+
+def shortened(t):
+    t = t.clone()
+    t.untyped_storage().resize_(t.untyped_storage().nbytes() - 1)
+    return t
+
+
+def misaligned(t):
+    return torch.frombuffer(bytearray(t.numel() * t.element_size() + 1), dtype=t.dtype, offset=1).view(t.shape)
+
+
+def fake(t):
+    with FakeTensorMode():
+        return torch.empty(t.shape, dtype=t.dtype)
+
+
+def functional(t):
+    return torch._to_functional_tensor(t)
+
+
+KINDS = {
+    "fake": fake,
+    "functional": functional,
+    "zeros": lambda t: torch._efficientzerotensor(t.shape, dtype=t.dtype),
+    "negated": torch._neg_view,
+    "masked": masked,
+    "freed": freed,
+    "shortened": shortened,
+    "misaligned": misaligned,
+    "sparse": lambda t: t.to_sparse(),
+}
+F8 = torch.float8_e4m3fn
+
+
+def arguments():
+    return dict(x=torch.ones(4, 256), dy=torch.ones(4, 256), scales=torch.ones(4, 2), codes=torch.ones(4, 256).to(F8),
+                weight=torch.ones(256), bias=torch.ones(256), mean=torch.zeros(4), rstd=torch.ones(4), shift=torch.zeros(4))
+
+
+CALLS = {
+    "forward": (lambda a: layer_norm_forward(a["x"], a["weight"], a["bias"]), ["x", "weight", "bias"]),
+    "forward of codes": (lambda a: layer_norm_forward(a["codes"], a["weight"], scales=a["scales"], dtype=torch.float32),
+                         ["codes", "scales", "weight"]),
+    "backward": (lambda a: layer_norm_backward(a["dy"], KeptRows(a["x"], None, a["mean"], a["rstd"], a["shift"]), a["weight"]),
+                 ["dy", "x", "mean", "rstd", "shift", "weight"]),
+    "backward of codes": (lambda a: layer_norm_backward(a["dy"], KeptRows(a["codes"], a["scales"], None, a["rstd"]), a["weight"]),
+                          ["dy", "codes", "scales", "rstd", "weight"]),
+    "save": (lambda a: save_fp8(a["x"]), ["x"]),
+    "restore": (lambda a: restore_fp8(a["codes"], a["scales"]), ["codes", "scales"]),
+    "weight gradient": (lambda a: fp8_weight_grad(a["dy"], a["codes"], a["scales"], a["weight"], a["bias"]),
+                        ["dy", "codes", "scales", "weight", "bias"]),
+}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("call", CALLS)
+def test_tensors_without_plain_memory_are_refused(call, kind):
+    """Their pointers are null or past their end, or their values are not what lies there."""
+    run, names = CALLS[call]
+    with pytest.raises(ValueError, match="on a GPU"):  # nothing else is wrong
+        run(arguments())
+    for name in names:
+        given = arguments()
+        if given[name].dtype == F8 and kind in ("negated", "masked", "sparse", "functional", "misaligned"):
+            continue  # there is no such tensor of codes
+        given[name] = KINDS[kind](given[name])
+        with pytest.raises((ValueError, RuntimeError)) as refusal:
+            run(given)
+        assert "on a GPU" not in str(refusal.value), name
