@@ -6,6 +6,7 @@
 #include <ATen/TracerMode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
@@ -38,8 +39,11 @@ void need(bool ok, const char *what) {
 
 // A trace (torch.jit.trace) does not see these calls and would keep their results
 // as constants.  `recorded`: the caller is an autograd function, which a trace
-// records as a whole.
+// records as a whole (a graph of the dispatcher's calls, make_fx, does not).
 void need_untraced(bool recorded) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    check(!Modes::any_modes_set() || !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+          "a graph of the dispatcher's calls would keep this call's result as a constant");
     check(recorded || !at::tracer::impl::is_dispatch_enabled(),
           "a trace would keep this call's result as a constant; trace layer_norm, linear or norm_linear");
 }

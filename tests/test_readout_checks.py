@@ -7,9 +7,21 @@ import pytest
 import torch
 import torch.masked
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from engram_rdma_lab_b200 import _native
-from engram_rdma_lab_b200.ops import KeptRows, check_readout, fp8_weight_grad, layer_norm_backward, layer_norm_forward, restore_fp8, save_fp8
+from engram_rdma_lab_b200.ops import (
+    KeptRows,
+    check_readout,
+    fp8_weight_grad,
+    layer_norm,
+    layer_norm_backward,
+    layer_norm_forward,
+    linear,
+    norm_linear,
+    restore_fp8,
+    save_fp8,
+)
 
 pytestmark = pytest.mark.skipif(not _native.available(), reason="extension not built")
 
@@ -130,3 +142,18 @@ def test_tensors_without_plain_memory_are_refused(call, kind):
         with pytest.raises((ValueError, RuntimeError)) as refusal:
             run(given)
         assert "on a GPU" not in str(refusal.value), name
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("call", [*CALLS, "layer_norm", "linear", "norm_linear"])
+def test_a_graph_of_the_dispatcher_is_refused(call):
+    """make_fx on real tensors would not see the calls, in autograd functions neither, and keep constants."""
+    a = arguments()
+    forms = {
+        "layer_norm": lambda x: layer_norm(x, a["weight"].requires_grad_(), a["bias"]),
+        "linear": lambda x: linear(x, torch.ones(8, 256, requires_grad=True)),
+        "norm_linear": lambda x: norm_linear(x, a["weight"].requires_grad_(), a["bias"], torch.ones(8, 256)),
+    }
+    run = forms.get(call) or (lambda x: CALLS[call][0](a)[0])
+    with pytest.raises(RuntimeError, match="constant"):
+        make_fx(run)(a["x"])
