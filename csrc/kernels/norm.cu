@@ -434,15 +434,28 @@ __global__ void __launch_bounds__(T0, 1024 / T0)
     }
 }
 
+// What a row's normalised values take beside its elements (exact rows).
+struct RowStats {
+    float mean = 0.f, shift = 0.f, rstd = 0.f;
+    __device__ __forceinline__ RowStats(const NormBackwardParams &p, int64_t r) {
+        if (p.keep != kKeepStats)
+            return;
+        mean = p.mean[r];
+        shift = p.shift != nullptr ? p.shift[r] : 0.f;
+        rstd = p.rstd[r];
+    }
+};
+
 // A normalised value of the backward pass.
-template <uint32_t X> __device__ __forceinline__ float kept_value(const NormBackwardParams &p, int64_t r, uint32_t c) {
+template <uint32_t X>
+__device__ __forceinline__ float kept_value(const NormBackwardParams &p, int64_t r, uint32_t c, const RowStats &row) {
     if (X == kE4m3)
         return Element<kE4m3>::get(p.codes[r * p.codes_stride + c]) *
                p.code_scales[r * p.code_scales_stride + c / kCheckpointBlock * p.scale_col_stride];
     else
-        return (Element<X>::get(static_cast<const typename Element<X>::T *>(p.x)[r * p.x_stride + c]) - p.mean[r] -
-                (p.shift != nullptr ? p.shift[r] : 0.f)) *
-               p.rstd[r];
+        return (Element<X>::get(static_cast<const typename Element<X>::T *>(p.x)[r * p.x_stride + c]) - row.mean -
+                row.shift) *
+               row.rstd;
 }
 
 template <uint32_t X, uint32_t DY>
@@ -456,13 +469,14 @@ __global__ void __launch_bounds__(kRowThreads) norm_backward_rows_any(const __gr
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
         const auto *dy = static_cast<const typename Element<DY>::T *>(p.dy) + r * p.dy_stride;
         auto *dx = static_cast<typename Element<DY>::T *>(p.dx) + r * p.width;
+        const RowStats row(p, r);
         float a = 0.f, b = 0.f;
         for (uint32_t c = threadIdx.x; c < p.width; c += kRowThreads) {
             float g = Element<DY>::get(dy[c]);
             if (p.weight != nullptr)
                 g *= load_param(p.weight, p.param_type, c);
             a += g;
-            b += g * kept_value<X>(p, r, c);
+            b += g * kept_value<X>(p, r, c, row);
         }
         const float2 sums = block_sum2(a, b, s_sum[turn]);
         const float c1 = sums.x * inv, c2 = sums.y * inv, rstd = p.rstd[r];
@@ -470,7 +484,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_backward_rows_any(const __gr
             float g = Element<DY>::get(dy[c]);
             if (p.weight != nullptr)
                 g *= load_param(p.weight, p.param_type, c);
-            dx[c] = Element<DY>::put(rstd * (g - c1 - kept_value<X>(p, r, c) * c2));
+            dx[c] = Element<DY>::put(rstd * (g - c1 - kept_value<X>(p, r, c, row) * c2));
         }
     }
 }
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_backward_columns_any(const _
         for (int64_t r = first + warp; r < last; r += kRowWarps) {
             const float g = Element<DY>::get(static_cast<const typename Element<DY>::T *>(p.dy)[r * p.dy_stride + c]);
             db += g;
-            dw += g * kept_value<X>(p, r, c);
+            dw += g * kept_value<X>(p, r, c, RowStats(p, r));
         }
     s_w[warp][lane] = dw;
     s_b[warp][lane] = db;

@@ -118,9 +118,10 @@ constexpr int64_t kPartBytes = 512 << 20;    // workspace for parts of the rows
 // Stages of the rows that one accumulator takes, four additions each.  What the
 // cuts of its additions take grows with their number, 7e-9 of the result's norm
 // for each: 3.7e-6 for 8192 rows.  A 16-bit result loses 1.7e-3 to its rounding
-// anyway; an fp32 one goes by 2048 rows, 6.5e-7 whatever their number (8192 x
-// 12288 to 2048: bf16 dy 512 us, 289 in one accumulator; fp32 dy 1014 us).
-__host__ __device__ constexpr uint32_t most_steps(uint32_t out_type) { return out_type == kFp32 ? 32 : 128; }
+// anyway; an fp32 one of 16-bit gradients goes by 4096 rows, of fp32 gradients by
+// 2048, 6.5e-7 whatever their number (8192 x 12288 to 2048: 970 us, 906 in one
+// accumulator for each term).
+uint32_t most_steps(uint32_t dy_type, uint32_t out_type) { return out_type != kFp32 ? 128 : dy_type != kFp32 ? 64 : 32; }
 constexpr int kLoadStages = 4, kOperandStages = 3;
 constexpr uint32_t kDyChunk = kSteps * 128;  // 64 columns of dy (bf16)
 constexpr uint32_t kCodeChunk = kSteps * 64; // 64 columns of codes
@@ -571,24 +572,57 @@ __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     }
 }
 
-// Adds the parts of the rows in order, and folds the norm in with the last.
-__global__ void __launch_bounds__(kThreads) weight_grad_join(const __grid_constant__ WeightGradParams p) {
-    const int64_t total = int64_t(p.out) * p.width, stride = int64_t(gridDim.x) * kThreads;
-    for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < total; at += stride) {
-        float v = 0.f;
-        for (uint32_t slot = 0; slot < p.joined; ++slot)
-            v += p.dw_parts[slot * total + at];
-        if (!p.last) {
-            p.dw_parts[at] = v;
-            continue;
+// Adds the parts of the rows in order, and folds the norm in with the last.  A
+// thread takes four adjacent columns of every gridDim.y-th output (by one load
+// and store where VECTOR).
+template <bool VECTOR> __global__ void __launch_bounds__(kThreads) weight_grad_join(const __grid_constant__ WeightGradParams p) {
+    const uint32_t k = (blockIdx.x * kThreads + threadIdx.x) * 4;
+    if (k >= p.width)
+        return;
+    const int64_t total = int64_t(p.out) * p.width;
+    float w[4], b[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        w[e] = p.last && p.norm_weight != nullptr && k + e < p.width ? load_param(p.norm_weight, p.param_type, k + e) : 1.f;
+        b[e] = p.last && p.norm_bias != nullptr && k + e < p.width ? load_param(p.norm_bias, p.param_type, k + e) : 0.f;
+    }
+    for (uint32_t o = blockIdx.y; o < p.out; o += gridDim.y) {
+        const int64_t at = int64_t(o) * p.width + k;
+        float v[4] = {};
+#pragma unroll 4
+        for (uint32_t slot = 0; slot < p.joined; ++slot) {
+            const float *part = p.dw_parts + slot * total + at;
+            if constexpr (VECTOR) {
+                const float4 q = *reinterpret_cast<const float4 *>(part);
+                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (k + e < p.width)
+                        v[e] += part[e];
+            }
         }
-        const int64_t o = at / p.width;
-        const uint32_t k = uint32_t(at - o * p.width);
-        if (p.norm_weight != nullptr)
-            v *= load_param(p.norm_weight, p.param_type, k);
-        if (p.norm_bias != nullptr)
-            v += load_param(p.norm_bias, p.param_type, k) * p.dy_sums[o];
-        store_param(p.dweight, p.out_type, at, v);
+        if (p.last) {
+            const float sum = p.norm_bias != nullptr ? p.dy_sums[o] : 0.f;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                if (p.norm_weight != nullptr)
+                    v[e] = __fmul_rn(v[e], w[e]);
+                if (p.norm_bias != nullptr)
+                    v[e] = __fmaf_rn(b[e], sum, v[e]);
+            }
+        }
+        const uint32_t type = p.last ? p.out_type : uint32_t(kFp32);
+        void *to = p.last ? p.dweight : p.dw_parts;
+        if (VECTOR && type == kFp32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(to) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else if (VECTOR)
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(to) + at) =
+                type == kBf16 ? make_uint2(to_bf16x2(v[0], v[1]), to_bf16x2(v[2], v[3]))
+                              : make_uint2(to_fp16x2(v[0], v[1]), to_fp16x2(v[2], v[3]));
+        else
+            for (uint32_t e = 0; e < 4 && k + e < p.width; ++e)
+                store_param(to, type, at + e, v[e]);
     }
 }
 
@@ -638,7 +672,7 @@ void plan_weight_grad(WeightGradParams &p, int num_sms) {
     // operands in, and out for each half); the epilogue moves ~12 values a cycle
     // and block.  Splitting the rows costs a pass over the parts at ~3.5 KB a cycle.
     double best = 1e300;
-    const int64_t limit = most_steps(p.out_type), fewest = (steps + limit - 1) / limit;
+    const int64_t limit = most_steps(p.type, p.out_type), fewest = (steps + limit - 1) / limit;
     const int64_t most = std::max(fewest, std::min<int64_t>(steps, 64));
     for (uint32_t tile = 32; tile <= 256; tile += 32) {
         const uint32_t tiles_k = (p.width + tile - 1) / tile;
@@ -706,8 +740,13 @@ cudaError_t launch_weight_grad(const WeightGradParams &p, cudaStream_t stream) {
         q.joined = q.first_slot + count;
         q.last = first == p.parts;
         if (p.parts > 1) {
-            const int64_t need = (int64_t(p.out) * p.width + kThreads - 1) / kThreads;
-            weight_grad_join<<<uint32_t(std::min<int64_t>(need, 148 * 16)), kThreads, 0, stream>>>(q);
+            // Blocks enough to fill the GPU, or one for each output.
+            const uint32_t across = (p.width + 4 * kThreads - 1) / (4 * kThreads);
+            const dim3 blocks(across, std::max(1u, std::min({p.out, 148 * 16 / across + 1, 65535u})));
+            if (p.width % 4 == 0)
+                weight_grad_join<true><<<blocks, kThreads, 0, stream>>>(q);
+            else
+                weight_grad_join<false><<<blocks, kThreads, 0, stream>>>(q);
         }
     }
     return cudaGetLastError();

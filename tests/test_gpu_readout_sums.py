@@ -44,8 +44,8 @@ def test_weight_grad_holds_all_terms_of_a_gradient(m, dtype):
 @pytest.mark.parametrize("signs", ["one", "both"])
 @pytest.mark.parametrize("m,n,out", [(8192, 256, 136), (262_144, 256, 264)])
 def test_weight_grad_of_very_many_rows(m, n, out, signs, dtype):
-    """An accumulator of an fp32 result takes 2048 rows, 16 at a time (those of smaller terms of dy before add 2^-7 of
-    it), before it is rounded into the sum of its like.  A cut is U of the accumulator on average, which grows linearly
+    """An accumulator of an fp32 result takes 2048 rows of fp32 or 4096 of bf16, 16 at a time (those of smaller terms of
+    dy before add 2^-7 of it), before it is rounded into the sum of its like.  A cut is U of the accumulator on average, which grows linearly
     (1/2 of its last size on average) where all terms have one sign, as a square root (2/3) otherwise; joining p
     parts rounds p times, half a U each."""
     x, dy = randn(m, m, n), randn(m + 1, m, out)
@@ -57,7 +57,8 @@ def test_weight_grad_of_very_many_rows(m, n, out, signs, dtype):
     for at in range(0, m, 65536):
         want = want + dy[at:at + 65536].double().t() @ rows[at:at + 65536]
     got, sums = fp8_weight_grad(dy, codes, scales, dtype=FP32)
-    bound = 1.02 * 128 * U * (1 / 2 if signs == "one" else 2 / 3) + m / 2048 / 2 * U
+    most = 2048 if dtype == FP32 else 4096
+    bound = 1.02 * (most / 16) * U * (1 / 2 if signs == "one" else 2 / 3) + m / most / 2 * U
     assert (got.double() - want).norm() <= bound * want.norm()
     # Column sums of dy: 32 parts of m / 32 rows by eight warps, then 8 + 32 additions.
     total = dy.double().sum(0)
