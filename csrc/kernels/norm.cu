@@ -40,7 +40,8 @@ __device__ __forceinline__ float row_rstd(float variance, float eps) {
 // that underflowed, and no eps) or NaN, none of a row's values is finite: scale
 // 1, and 2^-k as NaN makes every code NaN, where the conversion would saturate.
 __device__ __forceinline__ BlockScale kept_scale(float amax, float rstd) {
-    return rstd <= FLT_MAX ? block_scale(amax) : BlockScale{1.f, __uint_as_float(0x7FFFFFFFu)};
+    const BlockScale s = block_scale(rstd <= FLT_MAX ? amax : 0.f);
+    return {s.up, fmaf(rstd, 0.f, s.down)};
 }
 
 // One element of a forward row as fp32.
