@@ -53,8 +53,8 @@ template <uint32_t TYPE> __device__ __forceinline__ Raw8<TYPE> load_values8(cons
 
 // Rows of whole 16-column chunks on 16-byte boundaries: a lane turns 16 values
 // into one 16-byte store of codes; eight lanes hold a block.  8192 x 12288 bf16:
-// 49.8 us, 6.07 TB/s (0.92 of a copy's rate); one value per lane and load took
-// 157 us.
+// 53.2 us, 5.7 TB/s (0.86 of a copy's rate; 49.8 us without the call before it);
+// one value per lane and load took 157 us.
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) save_chunks(const __grid_constant__ SaveFp8Params p) {
     const uint32_t lane = threadIdx.x % 32, blocks = (p.width + kCheckpointBlock - 1) / kCheckpointBlock;
@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kThreads) save_chunks(const __grid_constant__ 
 
 // Any width, stride and alignment: a warp takes blocks of 128 columns, a lane
 // four adjacent ones, whose codes leave in one store (rows of codes start on
-// 16-byte boundaries).  4096 x 4097 bf16: 30 us, 1.7 TB/s.
+// 16-byte boundaries).  4096 x 4097 bf16: 33 us, 1.5 TB/s, bound by the number of
+// loads (one element each).
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) save_any(const __grid_constant__ SaveFp8Params p) {
     const uint32_t lane = threadIdx.x % 32;
@@ -169,7 +170,7 @@ template <uint32_t TYPE> __device__ __forceinline__ float held(float v, float sc
     return isnan(v) || isinf(scale) ? v : fminf(fmaxf(v, -most), most);
 }
 
-// The way back: 8192 x 12288 to bf16 in 54.8 us, 5.5 TB/s (two thirds of what it
+// The way back: 8192 x 12288 to bf16 in 57.8 us, 5.2 TB/s (two thirds of what it
 // moves are stores, 32 bytes per lane; as 16-byte stores they took 72 us).
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) restore_chunks(const __grid_constant__ RestoreFp8Params p) {
@@ -222,6 +223,8 @@ __global__ void __launch_bounds__(kThreads) restore_chunks(const __grid_constant
     }
 }
 
+// Any width, stride and alignment, by bytes and elements: 4096 x 4097 to bf16 29 us,
+// 1.7 TB/s.
 template <uint32_t TYPE>
 __global__ void __launch_bounds__(kThreads) restore_any(const __grid_constant__ RestoreFp8Params p) {
     const uint32_t lane = threadIdx.x % 32;

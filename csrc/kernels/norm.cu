@@ -67,7 +67,8 @@ template <> struct RowReader<kE4m3> {
 
 // Any width, stride and alignment: one block per row, which it reads three
 // times (twice from cache).  What takes it: rows past 16384 columns, and codes
-// whose rows, entries or scale blocks are not whole vectors.
+// whose rows, entries or scale blocks are not whole vectors.  4096 x 20001 bf16:
+// 325 us, 1.0 TB/s.
 template <uint32_t IN, uint32_t OUT>
 __global__ void __launch_bounds__(kRowThreads) norm_forward_any(const __grid_constant__ NormForwardParams p) {
     __shared__ WarpSums s_sum[2];
@@ -169,10 +170,12 @@ __device__ __forceinline__ void give_up(uint64_t *full, int depth, uint32_t slot
 // output.  Sixteen lanes hold a checkpoint block, so its largest value takes
 // four shuffles.  Four chunks per thread: with two, the two sums (a barrier and
 // ten shuffles each) were shared by half as many values.  8192 x 12288 bf16 with
-// 8 bits kept: 98 us, 5.1 TB/s; 4096 x 6144: 22.6 us, 4.4 TB/s; from e4m3 rows
-// 23.4 us, 3.2 TB/s.  Bound by issue slots: they are taken 45-60% of the time
-// (decoding, the parameters' conversion, sums) with 24 warps per SM, which is
-// what 80 registers allow; 64 registers and 30 warps spilled and were slower.
+// 8 bits kept: 102 us, 4.9 TB/s; 4096 x 6144 bf16: 24.8 us, 4.1 TB/s; from e4m3
+// rows 26.1 us, 2.9 TB/s (33.1 kept).  Bound by latency at few warps: 80 registers
+// allow 24 per SM, and with them issue slots are free 41% of the time while warps
+// wait for loads from L1 and shared memory (37% of their time), for the latency of
+// the instruction before (17%) and at barriers (8%).  64 registers and 30
+// warps spilled and were 4-8% slower.
 template <uint32_t IN, uint32_t OUT, uint32_t PARAM, int V, bool FULL, bool FP8, int T>
 __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
     norm_forward_row(const __grid_constant__ NormForwardParams p, bool warp_rows) {
@@ -337,9 +340,10 @@ __global__ void __launch_bounds__(T, T > 384 ? 1 : 768 / T)
 // Rows of 16- and 32-bit values of any width up to 16384 and any alignment, one
 // read: as above with single values for chunks, so every access is one element
 // (64 or 128 bytes of a warp together).  E is a multiple of four: a warp's
-// columns are whole checkpoint blocks.  4096 x 4097 bf16: 39 us, 1.7 TB/s, bound
-// by issue slots (with eight elements per thread the sums' share made it 52 us;
-// reading the row three times took 56 us).
+// columns are whole checkpoint blocks.  4096 x 4097 bf16: 43 us, 1.5 TB/s, 8
+// bits kept 60 us: an access moves one element, and a thread's sixteen spill 70-90
+// bytes of 64 registers where codes are kept (with eight elements per thread the
+// sums' share made it a third slower; reading the row three times 45% slower).
 template <uint32_t IN, uint32_t PARAM, int E, bool FP8, int T0>
 __global__ void __launch_bounds__(T0, 1024 / T0)
     norm_forward_elements(const __grid_constant__ NormForwardParams p, bool warp_rows) {
@@ -492,7 +496,8 @@ __global__ void __launch_bounds__(kRowThreads) norm_backward_rows_any(const __gr
 
 // Past 12288 columns of what norm_backward_row does not take: dx by a block per
 // row, then column sums of dy and dy h over one part of the rows: a block takes
-// 32 columns, its warps every eighth row of the part.
+// 32 columns, its warps every eighth row of the part.  4096 x 20001 bf16 exact: 646
+// us, 0.76 TB/s (rows are read three times).
 template <uint32_t X, uint32_t DY>
 __global__ void __launch_bounds__(kRowThreads) norm_backward_columns_any(const __grid_constant__ NormBackwardParams p) {
     __shared__ float s_w[kRowWarps][32], s_b[kRowWarps][32];
@@ -550,9 +555,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_backward_join(const __gr
 // part of them.  A ring slot holds dy's row, then the kept one, each with room
 // for a chunk in every place; what no chunk fills is zero and adds nothing.
 // Both passes over a row read it from the ring: holding it in registers beside
-// the sums left one block per SM.  8192 x 12288 from 8 bits: 94 us, 5.33 TB/s
-// (0.81 of a copy's rate); 4096 x 6144 bf16 exact: 31 us, 4.9 TB/s, 4-5 us of
-// them the join of the parts.
+// the sums left one block per SM.  8192 x 12288 from 8 bits: 99 us, 5.1 TB/s
+// (0.78 of a copy's rate); 4096 x 6144 bf16 exact: 35 us, 4.3 TB/s, 4-5 us of
+// them the join of the parts.  Bound by latency at few warps: 154-168 registers
+// leave 12 per SM at widths of 6144 and 12288, 7 to 9 between 6152 and 9216 (4096
+// rows from 8 bits: 6144 34.7 us, 7168 45.4, 8192 46.4, 9216 53.6), and issue slots
+// are free half of the time.  Past 12288 columns 512 threads of 128 registers spill
+// 90-150 bytes.
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int V, int T>
 __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
     constexpr int kDepth = ring_depth(DY);
@@ -731,8 +740,10 @@ __global__ void __launch_bounds__(T) norm_backward_row(const __grid_constant__ N
 }
 
 // The same for rows of up to 12288 columns of any alignment, by single elements.
-// 4096 x 4097 bf16: 58 us, 1.7 TB/s (two passes over the rows took 111 us); a
-// branch around each load made it 83 us, from 8 bits 192 us.
+// 4096 x 4097 bf16: 62 us, 1.6 TB/s (two passes over the rows took 111 us); a
+// branch around each load made it 83 us, from 8 bits 192 us.  Bound by the number
+// of accesses, and by spills: 8-36 bytes of 64 registers up to 4096 columns, 240-370
+// of 80 past 8192 (8192 x 11111 from 8 bits 286 us, 1.6 TB/s).
 template <uint32_t X, uint32_t DY, uint32_t PARAM, int E, int T>
 __global__ void __launch_bounds__(T, E == 8 ? 2 : 1) norm_backward_elements(const __grid_constant__ NormBackwardParams p, bool warp_rows) {
     using D = typename Element<DY>::T;
@@ -864,7 +875,8 @@ cudaError_t forward_row(const NormForwardParams &p, int num_sms, cudaStream_t st
 
 template <uint32_t IN, uint32_t OUT, uint32_t PARAM>
 cudaError_t forward_rows(const NormForwardParams &p, int num_sms, cudaStream_t stream) {
-    // By the width alone, so a row's bits do not depend on its batch.
+    // By the width alone (and whole_chunks, by alignment), never by the number of rows:
+    // a row's bits do not depend on its batch.
     const uint32_t chunks = p.width / 8;
     return chunks <= 32        ? forward_row<IN, OUT, PARAM, 1, false, 128>(p, num_sms, stream)
            : chunks <= 64      ? forward_row<IN, OUT, PARAM, 2, false, 128>(p, num_sms, stream)

@@ -8,15 +8,15 @@
 //
 // X is decoded to bf16 on its way into shared memory, which is exact: a code
 // has four significant bits and its scale is a power of two.  dy is bf16, or a
-// sum of bf16 terms that hold every bit of it (two for fp16, three for fp32),
-// one more pass over the rows for each.  So all products are exact and only
+// sum of bf16 terms that hold every bit of it down to 2^-133 (two for fp16, three
+// for fp32), one more pass over the rows for each.  So all products are exact and only
 // the fp32 accumulation rounds.  The tensor core cuts what it adds rather than
 // rounding it, an error that goes with the accumulator's size and the number of
 // additions: the smallest terms go first, while the accumulator is small (512
 // rows of fp32 are 1.5e-7 of the result's norm off, with the largest term first
-// they were 2.5e-6), and an accumulator takes a limited number of rows before it is
-// rounded into the sum of its like (most_steps), so that the error does not grow
-// with the rows.
+// they were 2.5e-6), and an accumulator takes a limited number of rows before it
+// is rounded into the sum of its like (most_steps), so that the error does not
+// grow with the rows.
 #include <algorithm>
 
 #include "../driver.h"
@@ -300,12 +300,12 @@ __device__ __forceinline__ void store_tile(const WeightGradParams &p, const CUte
 // stage for both halves; warp 11 adds up the column sums of dy meanwhile.
 // Accumulators fill TMEM (2 x 256 columns).
 //
-// 8192 x 12288 to 2048 bf16: 286 us, 1440 TFLOP/s (0.86 of the measured cuBLAS
-// burst; the library's product of the same size with bf16 rows at hand takes 260
-// us, and restoring them first 55 us more); 4096 x 6144 to 2048: 90 us, 1147
-// TFLOP/s: its 128 tiles are 1.7 rounds of the 74 pairs.  A round costs ~8 us
-// outside its MMAs (fill, epilogue), and a stage of 64 rows 1370 cycles for 896
-// of MMAs at the widest tile.
+// 8192 x 12288 to 2048 bf16: 291 us, 1417 TFLOP/s (0.85 of the measured cuBLAS
+// burst; the library's product of the same size with bf16 rows at hand takes 265
+// us, and restoring them first 58 us more); 4096 x 6144 to 2048 with a norm folded
+// in: 106 us, 970 TFLOP/s: its 128 tiles are 1.7 rounds of the 74 pairs.  A round
+// costs ~8 us outside its MMAs (fill, epilogue), and a stage of 64 rows 1370 cycles
+// for 896 of MMAs at 224 columns, the tile chosen for 8192 x 12288 to 2048.
 __global__ void __cluster_dims__(2) __launch_bounds__(kTensorThreads, 1)
     weight_grad_tensor(const __grid_constant__ WeightGradParams p, const __grid_constant__ CUtensorMap dy_map,
                        const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap out_map) {
