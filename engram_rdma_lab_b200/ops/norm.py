@@ -91,7 +91,7 @@ def layer_norm_backward(dy, kept: KeptRows, weight=None, *, want_dx: bool = True
     the weight's type; both are None without a ``weight``.  What is not wanted is None and not computed.
     """
     return _native.load().norm_backward(dy, kept.rows, kept.scales, kept.mean, kept.rstd, weight, want_dx, want_params,
-                                        kept.shift)
+                                        getattr(kept, "shift", None))
 
 
 def check_readout(device=None) -> None:
@@ -153,7 +153,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hid
                keep: str = "fp8"):
     """Differentiable layer norm of ``x [tokens, width]``; the arguments are :func:`layer_norm_forward`'s.
 
-    ``keep`` (``"fp8"`` or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
+    ``keep`` (``"fp8"``, also for fp32 rows, or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
     is wanted.  ``"exact"`` keeps ``x`` itself: rows that ``EngramBuffer.fetch`` returned last until the next fetch,
     after which the backward pass raises (not after the replay of a captured fetch, which nothing counts), so take
     ``"fp8"`` or a copy where fetches run ahead of backward passes.  There is no forward-mode derivative (a tangent raises).  Looked-up e4m3 codes get no gradient

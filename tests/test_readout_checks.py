@@ -2,6 +2,7 @@
 
 import copy
 import pickle
+import types
 
 import pytest
 import torch
@@ -157,3 +158,10 @@ def test_a_graph_of_the_dispatcher_is_refused(call):
     run = forms.get(call) or (lambda x: CALLS[call][0](a)[0])
     with pytest.raises(RuntimeError, match="constant"):
         make_fx(run)(a["x"])
+
+
+def test_kept_rows_of_another_kind_serve():
+    """Anything with the four fields does; the second part of the mean is then zeros."""
+    kept = types.SimpleNamespace(rows=torch.ones(4, 8), scales=None, mean=torch.zeros(4), rstd=torch.ones(4))
+    with pytest.raises(ValueError, match="on a GPU"):
+        layer_norm_backward(torch.ones(4, 8), kept)
