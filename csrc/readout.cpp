@@ -103,12 +103,18 @@ void need_plain(const Tensor &t) {
          "tensors must be plain, with their values in memory");
 }
 
-// The device all of these are on, which has to be a GPU.
-int need_device(const Tensor &first, std::initializer_list<const OptTensor *> others) {
-    need_plain(first);
+// The device all of these are on, which has to be a GPU.  Results carry no tangent
+// of forward-mode differentiation, so arguments may not either (`recorded`: an
+// autograd function's do, and torch raises for it).
+int need_device(const Tensor &first, std::initializer_list<const OptTensor *> others, bool recorded = false) {
+    const auto check_one = [recorded](const Tensor &t) {
+        need_plain(t);
+        need(recorded || !t._fw_grad(0).defined(), "the call would lose its arguments' tangents");
+    };
+    check_one(first);
     for (const OptTensor *t : others)
         if (*t)
-            need_plain(**t);
+            check_one(**t);
     need(first.is_cuda(), "tensors must be on a GPU");
     for (const OptTensor *t : others)
         need(!*t || (*t)->device() == first.device(), "tensors must be on one GPU");
@@ -217,7 +223,7 @@ py::tuple norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor
         need(!hidden, "hidden describes the scales of float8_e4m3fn rows");
     }
     need_params(weight, bias, width, out);
-    const int device = need_device(x, {&weight, &bias, &scales});
+    const int device = need_device(x, {&weight, &bias, &scales}, recorded);
     c10::cuda::CUDAGuard guard(device);
     const Tensor y = empty({rows, width}, out, x);
     OptTensor codes, code_scales, mean, rstd, shift;
@@ -343,7 +349,7 @@ py::tuple save_fp8(const Tensor &x, bool recorded) {
     need_untraced(recorded);
     need_rows(x, "activations must be [rows, width] with adjacent columns");
     need(is_wide(x.scalar_type()), "activations must be bfloat16, float16 or float32");
-    const int device = need_device(x, {});
+    const int device = need_device(x, {}, recorded);
     c10::cuda::CUDAGuard guard(device);
     const int64_t rows = x.size(0), width = x.size(1);
     const Tensor codes = empty_codes(x, rows, width), scales = empty_scales(x, rows, width);

@@ -8,9 +8,9 @@ value is exact in bf16.  Infinities and NaN come back as NaN and leave their blo
 Code rows start on 16-byte boundaries (``codes.stride(0)`` is the width rounded up to 16).
 
 ``restore_fp8`` gives the values back; :func:`~.norm.layer_norm_backward` and :func:`~.projection.fp8_weight_grad`
-read a checkpoint directly, which is cheaper.  Autograd sees neither call, and a trace is refused;
-:func:`~.projection.linear` and :func:`~.projection.norm_linear` are the differentiable forms that keep such a
-checkpoint.
+read a checkpoint directly, which is cheaper.  Autograd sees neither call (tangents of forward mode and traces are
+refused); :func:`~.projection.linear` and :func:`~.projection.norm_linear` are the differentiable forms that keep such
+a checkpoint.
 """
 
 from __future__ import annotations

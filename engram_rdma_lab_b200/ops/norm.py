@@ -78,8 +78,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, *, scales=N
     each looked-up row of ``hidden`` columns (default: the width); ``y`` is then ``dtype`` (default bf16).
     ``weight`` and ``bias [width]`` have y's type or are fp32.  ``keep`` says what the backward pass will read:
     nothing (``kept`` is None), ``"exact"`` (``x`` itself, which must stay unchanged) or ``"fp8"``.  Codes of a lookup
-    are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call, in
-    either mode, nor does a trace, which is refused (:func:`layer_norm` is their form).
+    are kept as ``"fp8"`` only: the next fetch reuses their memory.  Autograd does not see this call (tangents of
+    forward mode are refused), nor does a trace, which is refused (:func:`layer_norm` is their form).
     """
     return _forward(x, weight, bias, eps, scales, hidden, block, dtype, keep, False)
 
@@ -153,11 +153,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, scales=None, hid
                keep: str = "fp8"):
     """Differentiable layer norm of ``x [tokens, width]``; the arguments are :func:`layer_norm_forward`'s.
 
-    ``keep`` (``"fp8"``, also for fp32 rows, or ``"exact"``) chooses what is kept for the backward pass; nothing is kept where no gradient
-    is wanted.  ``"exact"`` keeps ``x`` itself: rows that ``EngramBuffer.fetch`` returned last until the next fetch,
-    after which the backward pass raises (not after the replay of a captured fetch, which nothing counts), so take
-    ``"fp8"`` or a copy where fetches run ahead of backward passes.  There is no forward-mode derivative (a tangent raises).  Looked-up e4m3 codes get no gradient
-    themselves (:func:`layer_norm_backward` gives their rows').
+    ``keep`` (``"fp8"``, also for fp32 rows, or ``"exact"``) chooses what is kept for the backward pass; nothing is
+    kept where no gradient is wanted.  ``"exact"`` keeps ``x`` itself: rows that ``EngramBuffer.fetch`` returned last
+    until the next fetch, after which the backward pass raises (not after the replay of a captured fetch, which nothing
+    counts), so take ``"fp8"`` or a copy where fetches run ahead of backward passes.  There is no forward-mode
+    derivative (a tangent raises).  Looked-up e4m3 codes get no gradient themselves (:func:`layer_norm_backward` gives
+    their rows').
     """
     if _keep_mode(keep) == 0:
         raise ValueError('keep must be "exact" or "fp8"')

@@ -27,9 +27,9 @@ def fp8_weight_grad(dy, codes, scales, norm_weight=None, norm_bias=None, *, dtyp
     ``X * norm_weight + norm_bias``.  Both results have dy's type, or ``dtype`` fp32; ``dbias`` is None without
     ``bias_grad``.  Products are exact (dy enters as bf16 terms that hold all of its bits down to 2^-133, the
     checkpoint's values are exact in bf16; scales that are no powers of two round them to bf16) and summed in fp32 on
-    the tensor cores, which cut what they add.  So no more than 2048 rows of an fp32 ``dy`` go into one sum, 4096 of a 16-bit one into an fp32
-    result, 8192 into a 16-bit result, and those sums are joined by rounded additions: fp32 results are 7e-7 and 2e-6
-    of their norm off, whatever the number of rows, 16-bit ones 4e-6 beside their rounding.
+    the tensor cores, which cut what they add.  So no more than 2048 rows of an fp32 ``dy`` go into one sum, 4096 of a
+    16-bit one into an fp32 result, 8192 into a 16-bit result, and those sums are joined by rounded additions: fp32
+    results are 7e-7 and 2e-6 of their norm off, whatever the number of rows, 16-bit ones 4e-6 beside their rounding.
     """
     return _native.load().fp8_weight_grad(dy, codes, scales, norm_weight, norm_bias, dtype, bias_grad)
 

@@ -6,6 +6,7 @@ import types
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.masked
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
@@ -165,3 +166,19 @@ def test_kept_rows_of_another_kind_serve():
     kept = types.SimpleNamespace(rows=torch.ones(4, 8), scales=None, mean=torch.zeros(4), rstd=torch.ones(4))
     with pytest.raises(ValueError, match="on a GPU"):
         layer_norm_backward(torch.ones(4, 8), kept)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_tangent_is_refused(call):
+    """The results of direct calls carry none, which would count as zero."""
+    run, names = CALLS[call]
+    for name in names:
+        with forward_ad.dual_level():
+            given = arguments()
+            if given[name].dtype == F8:
+                continue
+            given[name] = forward_ad.make_dual(given[name], torch.ones_like(given[name]))
+            with pytest.raises(ValueError, match="tangent"):
+                run(given)
+            with pytest.raises(ValueError, match="on a GPU"):  # an open level alone is none
+                run(arguments())
